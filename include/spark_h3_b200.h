@@ -385,6 +385,61 @@ int sb_fp8_quantize_segments(const void* x, int64_t M, int K, int seg, int64_t s
                              uint8_t* out, float* scales, void* stream);
 
 /*
+ * e4m3 quantisers with one scale per row and 128 columns (no counterpart in the reference, whose
+ * scales are per token or per tensor): for columns [128 b, 128 b + 128) of row m (the last block
+ * may be short), scales[m, b] = max(absmax * fp32(1/448), 1e-12) and out = e4m3(y * (1 / scale)),
+ * y being x, a * g * sigmoid(g) of a [M, 2K] projection output (value half first), or GELU(x)
+ * (erf form), evaluated in fp32.  A code equals e4m3(y / scale) except where that quotient lies
+ * within 2^-23 of itself from the middle of two codes.  A NaN makes its whole block NaN; an
+ * infinity makes its block's finite values 0.
+ * x: rows of K (swiglu: 2K) columns, x_stride elements apart (dtype); any alignment of its
+ * elements, 16-byte loads where every row starts on a 16-byte boundary and K % 8 == 0.
+ * out: [M, K] bytes; scales: [M, ceil(K / 128)] fp32.
+ */
+int sb_fp8_quantize_blocks(const void* x, int64_t x_stride, int dtype, int64_t M, int K, uint8_t* out,
+                           float* scales, void* stream);
+int sb_fp8_swiglu_quantize_blocks(const void* h, int64_t h_stride, int dtype, int64_t M, int K, uint8_t* out,
+                                  float* scales, void* stream);
+int sb_fp8_gelu_quantize_blocks(const void* x, int64_t x_stride, int dtype, int64_t M, int K, uint8_t* out,
+                                float* scales, void* stream);
+
+/*
+ * Residual addition, RMSNorm and e4m3 quantisation of each row in one pass (no counterpart in
+ * the reference):
+ *   s = residual + gate * x            (fp32; stored rounded to the dtype as `summed`)
+ *   y = s * rsqrt(mean(s^2) + eps) * weight + shift
+ *   out = e4m3(y * (1 / scale)),  scale = max(absmax(y) * fp32(1/448), 1e-12)
+ * with one scale per row (blocks 0, scales [M]: the operand of sb_fp8_gemm) or per row and 128
+ * columns (blocks 1, scales [M, ceil(C / 128)]: the operand of sb_fp8_gemm_blocks).  The norm
+ * works on the unrounded sum.  residual and summed are both NULL (s = x) or both given; summed
+ * ([M, C], contiguous) may be the residual itself when that is contiguous.  gate, weight and
+ * shift (fp32) may be NULL (1, 1, 0); row m uses row m / rows_per_sample of each, *_stride floats
+ * apart (0: one vector for all samples).  x, residual: rows of C elements (dtype), *_stride
+ * elements apart.  C <= 16384.
+ */
+int sb_fp8_add_rms_norm_quantize(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                 const float* gate, int64_t gate_stride, const float* weight, int64_t weight_stride,
+                                 const float* shift, int64_t shift_stride, int dtype, int64_t M, int C,
+                                 int64_t rows_per_sample, float eps, int blocks, void* summed, uint8_t* out,
+                                 float* scales, void* stream);
+
+/*
+ * e4m3 GEMM with one scale per 128 columns of K on both operands (no counterpart in the
+ * reference, whose GEMM takes per-row or per-tensor scales, fp8_linear.py:147-156):
+ *   out[m, n] = sum_b a_scale[m, b] * b_scale[n / 128, b] * sum_{k in block b} a[m, k] * b[n, k]
+ *               + bias[n],   and residual[m, n] + gate[n] * (that) with a residual.
+ * Blocks are summed in order of b in fp32 (where a few rows leave the GPU idle, K is split into
+ * up to 8 runs of blocks whose sums are added in order: a fixed choice by M, N and K).
+ * a: [M, K] e4m3; a_scale[m * a_row_stride + b * a_block_stride] fp32; b: [N, K] e4m3 (the
+ * weight, K-major); b_scale: [ceil(N / 128), ceil(K / 128)] fp32; bias, gate: [N] fp32 or NULL;
+ * residual: [M, N] of the output's type or NULL (it may be the output); a NULL gate is 1; out: [M, N]
+ * (out_dtype).  K must be a multiple of 16; a, b, residual and out 16-byte aligned.
+ */
+int sb_fp8_gemm_blocks(const uint8_t* a, const float* a_scale, int64_t a_row_stride, int64_t a_block_stride,
+                       const uint8_t* b, const float* b_scale, int64_t M, int N, int K, const float* bias,
+                       const void* residual, const float* gate, void* out, int out_dtype, void* stream);
+
+/*
  * DiT block pointwise stage (config 4): per row, y = x / rms(x) * (1 + scale) + shift (RMSNorm
  * with eps, adaLN modulation), quantised to e4m3 with one scale per row for the next GEMM.
  * x: [M, C] bf16, shift / scale: [C] fp32, out: [M, C] bytes, scales: [M] fp32.

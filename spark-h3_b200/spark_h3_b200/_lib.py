@@ -67,6 +67,12 @@ SIGNATURES = {
     "sb_fp8_gemm_residual": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _vp, _i, _vp]),
     "sb_fp8_gelu_quantize_rows": (_i, [_vp, _i, _i64, _i, _vp, _vp, _vp]),
     "sb_fp8_quantize_segments": (_i, [_vp, _i64, _i, _i, _i64, _vp, _vp, _vp]),
+    "sb_fp8_quantize_blocks": (_i, [_vp, _i64, _i, _i64, _i, _vp, _vp, _vp]),
+    "sb_fp8_swiglu_quantize_blocks": (_i, [_vp, _i64, _i, _i64, _i, _vp, _vp, _vp]),
+    "sb_fp8_gelu_quantize_blocks": (_i, [_vp, _i64, _i, _i64, _i, _vp, _vp, _vp]),
+    "sb_fp8_add_rms_norm_quantize": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i, _i64, _i, _i64, _f,
+                                          _i, _vp, _vp, _vp, _vp]),
+    "sb_fp8_gemm_blocks": (_i, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _i, _vp]),
     "sb_dit_norm_modulate_quantize": (_i, [_vp, _vp, _vp, _i64, _i, ctypes.c_float, _vp, _vp, _vp]),
     "sb_dit_qkv_norm_rope": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, ctypes.c_float, _vp, _vp, _vp, _vp]),
     "sb_memcpy2d": (_i, [_vp, _i64, _vp, _i64, _i64, _i64, _vp]),

@@ -1,7 +1,10 @@
 """e4m3 linears on the B200 tensor cores, with the module API of
 h3_sparse_attention/fp8_linear.py (`quantize_rows`, `quantize_tensor`, `swiglu_quantize`,
 `swiglu_quantize_tensor`, `Fp8Linear`, `forward_qkv_shared`, `Fp8SwiGLUFeedForward`,
-`Fp8AttnProcessor`, `convert_linear_to_fp8`, `install_fp8`).
+`Fp8AttnProcessor`, `convert_linear_to_fp8`, `install_fp8`), and a finer granularity beside it:
+one scale per token and 128 columns of the activation, one per 128 x 128 block of the weight
+(`quantize_blocks`, `swiglu_quantize_blocks`, `gelu_quantize_blocks`, `add_rms_norm_quantize`,
+`fp8_gemm_blocks`, `Fp8BlockLinear`; `install_fp8(..., scales="block")`).
 
 Scale granularity is per-token activation x per-output-channel weight on every card: the
 tcgen05 GEMM in libsparkh3b200.so applies both scale vectors in its epilogue, so the
@@ -23,12 +26,13 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from .ops import _dtype_code, _require_cuda, _stream
+from .ops import _dtype_code, _ptr, _require_cuda, _stream
 
 FP8_DTYPE = torch.float8_e4m3fn
 FP8_MAX = 448.0
 MIN_WIDTH = 4096
 SKIP_END_BLOCKS = 0
+BLOCK = 128  # columns (and weight rows) per scale of the block-scaled operators
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -104,6 +108,197 @@ def swiglu_quantize_tensor(h: torch.Tensor):
     return quantize_tensor(act)
 
 
+# ---------------------------------------------------------------- block scales
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _strided_rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
+    """x [M, C] with unit-stride, non-overlapping rows (copied when it has none) and the
+    distance between its rows."""
+    if x.dim() != 2:
+        raise ValueError(f"{name} must be [M, K], got {tuple(x.shape)}")
+    if not x.is_cuda:
+        raise RuntimeError("spark_h3_b200 kernels require CUDA tensors; there is no CPU path")
+    M, C = x.shape
+    if C == 0:
+        raise ValueError(f"{name} has no columns")
+    if x.stride(1) != 1 or (M > 1 and x.stride(0) < C):
+        x = x.contiguous()
+    return x, x.stride(0) if M > 1 else C
+
+
+def _same_device(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise RuntimeError(f"all tensors must be on the same CUDA device: {name} is on {t.device}, not {device}")
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """The C-ABI call with `device` current, on its current stream."""
+    stream = _stream(device)
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream)
+
+
+def _quantize_blocks(entry: str, x: torch.Tensor, halves: int):
+    x, stride = _strided_rows(x, "x")
+    dtype = _dtype_code(x)
+    M, K = x.shape
+    if K % halves:
+        raise ValueError(f"a [M, 2K] projection output is expected, got {tuple(x.shape)}")
+    K //= halves
+    y = torch.empty((M, K), device=x.device, dtype=FP8_DTYPE)
+    scale = torch.empty((M, _blocks(K)), device=x.device, dtype=torch.float32)
+    if M > 0:
+        _call_on(x.device, entry, x.data_ptr(), stride, dtype, M, K, y.data_ptr(), scale.data_ptr())
+    return y, scale
+
+
+def quantize_blocks(x: torch.Tensor):
+    """bf16/fp32 [M, K] -> (e4m3 [M, K], fp32 scales [M, ceil(K / 128)]): one absmax per row and
+    128 columns.  Rows may be strided (a column slice is read in place)."""
+    return _quantize_blocks("sb_fp8_quantize_blocks", x, 1)
+
+
+def swiglu_quantize_blocks(h: torch.Tensor):
+    """[M, 2K] projection output -> quantize_blocks(a * silu(gate)) with a, gate = h.chunk(2),
+    without writing the activation."""
+    return _quantize_blocks("sb_fp8_swiglu_quantize_blocks", h, 2)
+
+
+def gelu_quantize_blocks(x: torch.Tensor):
+    """quantize_blocks(gelu(x)) (erf form) without writing the activation."""
+    return _quantize_blocks("sb_fp8_gelu_quantize_blocks", x, 1)
+
+
+def _sample_vector(v: torch.Tensor | None, name: str, M: int, C: int, samples: int):
+    """A vector [C] or one per sample [S, C] as (fp32 tensor, stride between samples, S)."""
+    if v is None:
+        return None, 0, samples
+    if v.dim() not in (1, 2) or v.shape[-1] != C:
+        raise ValueError(f"{name} must be [{C}] or [samples, {C}], got {tuple(v.shape)}")
+    v = v.float()
+    if v.stride(-1) != 1 and C > 1:
+        v = v.contiguous()
+    if v.dim() == 1 or v.shape[0] == 1:
+        return v, 0, samples
+    S = v.shape[0]
+    if S == 0 or M % S or (samples not in (1, S)):
+        raise ValueError(f"{name} has {S} samples: {M} rows must split evenly among one number of samples")
+    return v, v.stride(0), S
+
+
+def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, *,
+                          gate: torch.Tensor | None = None, shift: torch.Tensor | None = None, eps: float = 1e-6,
+                          blocks: bool = True, out: torch.Tensor | None = None):
+    """s = residual + gate * x; y = s * rsqrt(mean(s^2) + eps) * weight + shift; y in e4m3.
+
+    x, residual: bf16/fp32 [M, C], C <= 16384, rows may be strided.  weight, gate, shift: [C],
+    or [S, C] with one row per sample (S divides M; row m belongs to sample m // (M / S)).
+    Returns (codes [M, C], scales, s): scales [M, ceil(C / 128)] (`blocks`, for fp8_gemm_blocks)
+    or [M, 1] (for fp8_gemm); s in x's dtype, written to `out` when given (which may be the
+    residual itself: the residual stream updated in place), or None without a residual.  The
+    norm works on the unrounded fp32 sum."""
+    x, x_stride = _strided_rows(x, "x")
+    device, dtype = x.device, _dtype_code(x)
+    M, C = x.shape
+    r_stride = 0
+    if residual is None:
+        if gate is not None or out is not None:
+            raise ValueError("gate and out belong to the residual's addition: pass a residual")
+    else:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"the residual must match x: {tuple(residual.shape)} {residual.dtype}, "
+                             f"not {tuple(x.shape)} {x.dtype}")
+        residual, r_stride = _strided_rows(residual, "residual")
+        if out is None:
+            out = torch.empty((M, C), device=device, dtype=x.dtype)
+        elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous {tuple(x.shape)} {x.dtype}")
+    _same_device(device, residual=residual, weight=weight, gate=gate, shift=shift, out=out)
+    samples = 1
+    gate, g_stride, samples = _sample_vector(gate, "gate", M, C, samples)
+    weight, w_stride, samples = _sample_vector(weight, "weight", M, C, samples)
+    shift, s_stride, samples = _sample_vector(shift, "shift", M, C, samples)
+    y = torch.empty((M, C), device=device, dtype=FP8_DTYPE)
+    scale = torch.empty((M, _blocks(C) if blocks else 1), device=device, dtype=torch.float32)
+    if M > 0:
+        _call_on(device, "sb_fp8_add_rms_norm_quantize", x.data_ptr(), x_stride, _ptr(residual), r_stride, _ptr(gate),
+                 g_stride, _ptr(weight), w_stride, _ptr(shift), s_stride, dtype, M, C, M // samples, eps, int(blocks),
+                 _ptr(out), y.data_ptr(), scale.data_ptr())
+    return y, scale, out
+
+
+def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Tensor, b_scale: torch.Tensor,
+                    bias: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
+                    gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """[M, N] = a_fp8 [M, K] . b_fp8 [N, K]^T with a_scale [M, ceil(K / 128)] (any strides) applied
+    per row and 128 columns and b_scale [ceil(N / 128), ceil(K / 128)] per 128 x 128 block
+    (+ bias [N]); residual + gate * (that) with a residual [M, N] of the output's dtype (gate [N],
+    1 when None).  out_dtype bf16 (the default) or fp32; `out` may be the residual itself."""
+    if a_fp8.dtype != FP8_DTYPE or b_fp8.dtype != FP8_DTYPE:
+        raise TypeError("fp8_gemm_blocks takes float8_e4m3fn operands")
+    if a_fp8.dim() != 2 or b_fp8.dim() != 2 or a_fp8.shape[1] != b_fp8.shape[1]:
+        raise ValueError(f"A [M, K] and B [N, K] must share K: {tuple(a_fp8.shape)} vs {tuple(b_fp8.shape)}")
+    if not a_fp8.is_cuda:
+        raise RuntimeError("spark_h3_b200 kernels require CUDA tensors; there is no CPU path")
+    device = a_fp8.device
+    _same_device(device, a_scale=a_scale, b_fp8=b_fp8, b_scale=b_scale, bias=bias, residual=residual, gate=gate, out=out)
+    a_fp8, b_fp8, b_scale = a_fp8.contiguous(), b_fp8.contiguous(), b_scale.contiguous()
+    (M, K), N = a_fp8.shape, b_fp8.shape[0]
+    for scale, rows, name in ((a_scale, M, "a_scale"), (b_scale, _blocks(N), "b_scale")):
+        if scale.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32")
+        if scale.shape != (rows, _blocks(K)):
+            raise ValueError(f"{name} must be [{rows}, {_blocks(K)}], got {tuple(scale.shape)}")
+    if out is not None:
+        out_dtype = out_dtype or out.dtype
+    elif out_dtype is None:
+        out_dtype = torch.bfloat16
+    if out is None:
+        out = torch.empty((M, N), device=device, dtype=out_dtype)
+    elif out.shape != (M, N) or out.dtype != out_dtype or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous [{M}, {N}] {out_dtype}")
+    code = _dtype_code(out)
+    if bias is not None:
+        bias = bias.float().contiguous()
+        if bias.numel() != N:
+            raise ValueError(f"bias needs {N} values, got {bias.numel()}")
+    if residual is not None:
+        if residual.shape != (M, N) or residual.dtype != out_dtype:
+            raise ValueError(f"the residual must be [{M}, {N}] {out_dtype}")
+        residual = residual.contiguous()
+        if gate is not None:
+            gate = gate.float().contiguous()
+            if gate.numel() != N:
+                raise ValueError(f"gate needs {N} values, got {gate.numel()}")
+    elif gate is not None:
+        raise ValueError("gate belongs to the residual's addition: pass a residual")
+    if M > 0 and N > 0:
+        _call_on(device, "sb_fp8_gemm_blocks", a_fp8.data_ptr(), a_scale.data_ptr(), a_scale.stride(0),
+                 a_scale.stride(1), b_fp8.data_ptr(), b_scale.data_ptr(), M, N, K, _ptr(bias), _ptr(residual),
+                 _ptr(gate), out.data_ptr(), code)
+    return out
+
+
+def quantize_weight_blocks(weight: torch.Tensor):
+    """e4m3 weight with one scale per 128 x 128 block: (codes [N, K], scales [ceil(N / 128),
+    ceil(K / 128)]), scale = max(absmax / 448, 1e-12) in fp32, codes = e4m3(weight / scale)."""
+    if weight.dim() != 2:
+        raise ValueError(f"expected a weight [N, K], got {tuple(weight.shape)}")
+    N, K = weight.shape
+    w = F.pad(weight.float(), (0, _blocks(K) * BLOCK - K, 0, _blocks(N) * BLOCK - N))
+    w = w.view(_blocks(N), BLOCK, _blocks(K), BLOCK)
+    scale = (w.abs().amax(dim=(1, 3)) / FP8_MAX).clamp_min(1e-12)
+    codes = (w / scale[:, None, :, None]).to(FP8_DTYPE).view(_blocks(N) * BLOCK, -1)
+    return codes[:N, :K].contiguous(), scale
+
+
 def quantize_activation(x: torch.Tensor):
     """What the GEMM callers use: per-token scales (the GEMM epilogue applies them)."""
     return quantize_rows(x)
@@ -175,24 +370,56 @@ class Fp8Linear(nn.Module):
         out = fp8_gemm(x_fp8, x_scale, self.weight_fp8, self.weight_scale, bias)
         return out if out_dtype == torch.bfloat16 else out.to(out_dtype)
 
+    # the activation quantisers whose scales this linear's GEMM takes
+    quantize = staticmethod(quantize_activation)
+    swiglu_quantize = staticmethod(swiglu_quantize_activation)
+
     def forward(self, x):
         shape = x.shape
         rows = x.reshape(-1, shape[-1])
-        out = self.forward_quantized(*quantize_activation(rows), out_dtype=rows.dtype)
+        out = self.forward_quantized(*self.quantize(rows), out_dtype=rows.dtype)
         return out.reshape(*shape[:-1], -1)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
 
+class Fp8BlockLinear(Fp8Linear):
+    """Fp8Linear with block scales: one per token and 128 columns of the activation, one per
+    128 x 128 block of the weight.  A large value then pushes only its own block's small values
+    into e4m3's subnormals.  Inference only, like Fp8Linear; in_features must be a multiple of 16."""
+
+    def __init__(self, linear: nn.Linear):
+        nn.Module.__init__(self)
+        if linear.in_features % 16:
+            raise ValueError(f"Fp8BlockLinear needs in_features in multiples of 16, got {linear.in_features}")
+        codes, scale = quantize_weight_blocks(linear.weight.detach())
+        self.register_buffer("weight_fp8", codes)
+        self.register_buffer("weight_scale", scale)
+        self.register_parameter("bias", linear.bias)
+        self.in_features = linear.in_features
+        self.out_features = linear.out_features
+
+    quantize = staticmethod(quantize_blocks)
+    swiglu_quantize = staticmethod(swiglu_quantize_blocks)
+
+    def forward_quantized(self, x_fp8, x_scale, out_dtype=torch.bfloat16):
+        """[M, K] e4m3 rows and their scales [M, ceil(K / 128)] -> [M, N]."""
+        bias = None if self.bias is None else self.bias.detach()
+        kernel_dtype = torch.float32 if out_dtype == torch.float32 else torch.bfloat16
+        out = fp8_gemm_blocks(x_fp8, x_scale, self.weight_fp8, self.weight_scale, bias, out_dtype=kernel_dtype)
+        return out if out_dtype == kernel_dtype else out.to(out_dtype)
+
+
 def forward_qkv_shared(attn, hidden_states):
-    """One quantisation of hidden_states feeds q/k/v when all three are Fp8Linear
-    (fp8_linear.py:296-310); None otherwise, and the caller runs the plain projections."""
+    """One quantisation of hidden_states feeds q/k/v when all three are Fp8Linear of one scale
+    granularity (fp8_linear.py:296-310); None otherwise, and the caller runs the plain
+    projections."""
     projections = (attn.to_q, attn.to_k, attn.to_v)
-    if not all(isinstance(p, Fp8Linear) for p in projections):
+    if not all(isinstance(p, Fp8Linear) and p.quantize is projections[0].quantize for p in projections):
         return None
     rows = hidden_states.reshape(-1, hidden_states.shape[-1])
-    x_fp8, x_scale = quantize_activation(rows)
+    x_fp8, x_scale = attn.to_q.quantize(rows)
     return tuple(p.forward_quantized(x_fp8, x_scale, out_dtype=hidden_states.dtype)
                  .reshape(*hidden_states.shape[:-1], -1) for p in projections)
 
@@ -213,7 +440,7 @@ class Fp8SwiGLUFeedForward(nn.Module):
     def forward(self, hidden_states):
         shape = hidden_states.shape
         h = self.proj(hidden_states.reshape(-1, shape[-1]))
-        out = self.down.forward_quantized(*swiglu_quantize_activation(h), out_dtype=h.dtype)
+        out = self.down.forward_quantized(*self.down.swiglu_quantize(h), out_dtype=h.dtype)
         return out.reshape(*shape[:-1], -1)
 
 
@@ -257,11 +484,15 @@ def _fuse_ff(block) -> bool:
     return True
 
 
-def convert_linear_to_fp8(model, min_width=MIN_WIDTH, skip_end_blocks=SKIP_END_BLOCKS):
+def convert_linear_to_fp8(model, min_width=MIN_WIDTH, skip_end_blocks=SKIP_END_BLOCKS, scales="channel"):
     """Swap the Linears at least `min_width` wide on both sides inside
     model.transformer_blocks for Fp8Linear, in place, and fuse each converted block's SwiGLU
     FeedForward (fp8_linear.py:398-427).  `skip_end_blocks` keeps the first and last N blocks
-    in bf16.  Returns how many Linears were swapped."""
+    in bf16.  `scales`: "channel" (per token x per output channel, Fp8Linear) or "block" (per
+    128 columns x per 128 x 128 block, Fp8BlockLinear).  Returns how many Linears were swapped."""
+    if scales not in ("channel", "block"):
+        raise ValueError(f'scales must be "channel" or "block", got {scales!r}')
+    kind = Fp8Linear if scales == "channel" else Fp8BlockLinear
     blocks = getattr(model, "transformer_blocks", None)
     if not blocks:
         raise ValueError("convert_linear_to_fp8 expects a model with a non-empty `transformer_blocks` ModuleList")
@@ -275,19 +506,19 @@ def convert_linear_to_fp8(model, min_width=MIN_WIDTH, skip_end_blocks=SKIP_END_B
                     continue
                 if child.in_features < min_width or child.out_features < min_width:
                     continue
-                setattr(parent, name, Fp8Linear(child).to(child.weight.device))
+                setattr(parent, name, kind(child).to(child.weight.device))
                 swapped += 1
         _fuse_ff(block)
     return swapped
 
 
-def install_fp8(pipe_or_transformer, min_width=MIN_WIDTH, skip_end_blocks=SKIP_END_BLOCKS):
+def install_fp8(pipe_or_transformer, min_width=MIN_WIDTH, skip_end_blocks=SKIP_END_BLOCKS, scales="channel"):
     """Convert a pipeline's (or a transformer's) wide block Linears, fuse the FeedForwards and
     install the shared-qkv processor on every converted attention (fp8_linear.py:430-447).
-    Call after the weights are loaded and before the sparse-attention plugin.  Returns how
-    many Linears were quantised."""
+    Call after the weights are loaded and before the sparse-attention plugin.  `scales` is the
+    granularity of convert_linear_to_fp8.  Returns how many Linears were quantised."""
     transformer = getattr(pipe_or_transformer, "transformer", pipe_or_transformer)
-    swapped = convert_linear_to_fp8(transformer, min_width=min_width, skip_end_blocks=skip_end_blocks)
+    swapped = convert_linear_to_fp8(transformer, min_width=min_width, skip_end_blocks=skip_end_blocks, scales=scales)
     for block in transformer.transformer_blocks:
         attn = getattr(block, "attn", None)
         if (attn is not None and not getattr(attn, "fused_projections", False)
