@@ -6,6 +6,8 @@
 // added with its scale to an fp32 accumulator in registers.
 #include <algorithm>
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -33,6 +35,7 @@ struct BlockGemmParams {
   const void* residual;   // optional [M, N], the output's type
   const float* gate;      // optional [N] (1), with a residual
   void* out;              // [M, N] bf16 or fp32
+  int a_vec;              // 1: a row's scales are consecutive and its first is 16-byte aligned
   int tma_out;            // 1: rows of whole 16-byte vectors, written by TMA stores
   int* status;
   int64_t M;
@@ -41,34 +44,54 @@ struct BlockGemmParams {
 };
 
 // ------------------------------------------------------------------ CTA-pair kernel
-// A cluster of two CTAs computes a 256 x 256 tile with tcgen05.mma.cta_group::2 (the pair's
-// operand and barrier protocol of fp8_gemm.cu), one k-block per stage and per TMEM buffer:
+// A cluster of two CTAs computes a 256 x 256 tile with tcgen05.mma.cta_group::2, one k-block per
+// stage.  A k-block's partial product goes to TMEM as two halves of 128 columns, each with its own
+// barriers, in two buffers: the issue of a half waits for the read-back of the half four issues
+// before it, and TMEM holds no more, so what counts is the time from a half's last MMA to its
+// next first one (the commit, the read-back, the arrival at rank 0) against the time of the
+// three halves between.  Halves shorten both the MMAs and the read-back in that loop.
 //   full[s]      rank 0 only: armed for both CTAs' bytes of a stage
 //   empty[s]     both CTAs: the MMA's commit releases the stage
-//   acc_full[b]  both CTAs: the commit after a k-block's four MMAs
-//   acc_empty[b] rank 0 only: one arrival per epilogue warp of both CTAs (16)
+//   acc_full[a]  both CTAs, a = 2 * buffer + half: the commit after a half's four MMAs
+//   acc_empty[a] rank 0 only: one arrival per epilogue warp of that half in both CTAs (8)
+//   scale_full[c], scale_empty[c]  per CTA: a chunk of 8 k-blocks' scales, from the scale warp to
+//                the epilogue warps
 //   mma_done     both CTAs: final commit, waited before TMEM is freed
-// Eight epilogue warps per CTA: warp w reads TMEM lanes 32 (w % 4) .. (its 32 rows) and columns
-// 128 (w / 4) .. (one weight block), so a k-block has ONE scale per thread, a_scale * b_scale.
-// The 128 accumulators of a thread stay in registers for the whole tile.
-constexpr int kPairThreads = 320;  // warps 0-7 epilogue, 8 TMA producer, 9 MMA issuer
-constexpr int kPairStages = 6;
+// Eight epilogue warps per CTA: warp w reads TMEM lanes 32 (w % 4) .. (its 32 rows) of half w / 4
+// (one weight block), so a k-block has ONE scale per thread, a_scale * b_scale.  The 128
+// accumulators of a thread stay in registers for the whole tile (setmaxnreg moves registers of
+// the other four warps to these eight).
+constexpr int kEpiWarps = 8;
+constexpr int kEpiThreads = 32 * kEpiWarps;
+constexpr int kProducerWarp = kEpiWarps, kIssuerWarp = kEpiWarps + 1, kScaleWarp = kEpiWarps + 2;
+constexpr int kPairThreads = kEpiThreads + 128;  // one warp idle
+constexpr int kLaunchRegs = 168, kEpiRegs = 208, kOtherRegs = 88;  // per thread
+static_assert(kEpiRegs * kEpiThreads + kOtherRegs * 128 == kLaunchRegs * kPairThreads,
+              "setmaxnreg redistributes exactly what the CTA was launched with");
+constexpr int kPairStages = 5;
+constexpr int kChunk = 8;  // k-blocks of scales per chunk; two chunks in shared memory
 constexpr int kPairOpBytes = 128 * kBlockK;       // one operand's 128 rows of a stage
 constexpr int kPairStageBytes = 2 * kPairOpBytes;  // A half + B half per CTA
-constexpr uint32_t kPairAccCols = 256;
-constexpr int kPairOutBox = 32 * 128;          // one epilogue warp's 32 rows x 128 bytes
-constexpr int kPairOutBytes = 8 * kPairOutBox;
+constexpr int kPairHalfBytes = 64 * kBlockK;      // a CTA's B rows of one half of the tile
+constexpr uint32_t kPairAccCols = 128;            // columns of a half; two halves x two buffers
+constexpr int kPairOutBox = 32 * 64;           // one epilogue warp's 32 rows x 64 bytes
+constexpr int kPairOutBytes = kEpiWarps * kPairOutBox;
+constexpr int kChunkFloats = kChunk * 2 * 128;  // [k-block][weight block of the tile][row]
+constexpr int kScaleBytes = 2 * kChunkFloats * 4;
 
 struct __align__(8) PairControl {
   uint64_t full[kPairStages], empty[kPairStages];
-  uint64_t acc_full[2], acc_empty[2];
+  uint64_t acc_full[4], acc_empty[4];
+  uint64_t scale_full[2], scale_empty[2];
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort_flag;
 };
 
+// Relaxed: what the arrival hands over are TMEM columns whose loads have completed (wait::ld); a
+// release would also wait for the thread's unrelated memory accesses.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster, int x,
                                                  int y) {
@@ -83,13 +106,16 @@ __device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t a_desc, ui
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar_cluster) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster)
-               : "memory");
+// Arrives on the barrier at the same offset of both CTAs.
+__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t holder_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(holder_smem), "r"(ncols)
@@ -114,29 +140,34 @@ __device__ __forceinline__ void tile_coords(int64_t t, int m_tiles, int n_tiles,
   nt = within / gm;
 }
 
-// Bias, gate and residual of `n` columns from column n0 of row m applied to f.
-template <typename T, int NCOLS>
-__device__ __forceinline__ void finish_columns(const BlockGemmParams& p, int64_t m, bool row_ok, int n0, float* f) {
+__device__ __forceinline__ void load16(const __nv_bfloat16* p, float* v) { load8_plain(p, v); }
+__device__ __forceinline__ void load16(const float* p, float* v) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+
+// Bias, gate and residual of the 16 bytes of output columns from column n of row m applied to f.
+// The residual may be the output: its loads are plain and precede the row's store.
+template <typename T>
+__device__ __forceinline__ void finish_columns(const BlockGemmParams& p, int64_t m, bool row_ok, int n, float* f) {
+  constexpr int kVec = 16 / (int)sizeof(T);
   if (p.bias != nullptr) {
 #pragma unroll
-    for (int i = 0; i < NCOLS; ++i)
-      if (n0 + i < p.N) f[i] += __ldg(p.bias + n0 + i);
+    for (int i = 0; i < kVec; ++i)
+      if (n + i < p.N) f[i] += __ldg(p.bias + n + i);
   }
   if (p.residual != nullptr && row_ok) {
-    const T* res = static_cast<const T*>(p.residual) + m * p.N + n0;
-    if (p.tma_out && n0 + NCOLS <= p.N) {
-#pragma unroll
-      for (int i = 0; i < NCOLS; i += 8) {
-        float r[8];
-        load8_plain(res + i, r);  // the output may be the residual
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[i + e] = fmaf(p.gate ? __ldg(p.gate + n0 + i + e) : 1.f, f[i + e], r[e]);
-      }
+    const T* res = static_cast<const T*>(p.residual) + m * p.N + n;
+    float r[kVec];
+    if (p.tma_out && n < p.N) {  // whole 16-byte vectors
+      load16(res, r);
     } else {
 #pragma unroll
-      for (int i = 0; i < NCOLS; ++i)
-        if (n0 + i < p.N) f[i] = fmaf(p.gate ? __ldg(p.gate + n0 + i) : 1.f, f[i], Elem<T>::to_f(res[i]));
+      for (int i = 0; i < kVec; ++i) r[i] = n + i < p.N ? Elem<T>::to_f(res[i]) : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (n + i < p.N) f[i] = fmaf(p.gate != nullptr ? __ldg(p.gate + n + i) : 1.f, f[i], r[i]);
   }
 }
 
@@ -148,7 +179,8 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   // Same layout in both CTAs, so both take the same branch here.
   const bool aligned = (smem_u32(smem) & 1023u) == 0u;
   uint8_t* sOut = smem + kPairStages * kPairStageBytes;  // output staging of the TMA stores
-  PairControl& C = *reinterpret_cast<PairControl*>(sOut + kPairOutBytes);
+  float* sScale = reinterpret_cast<float*>(sOut + kPairOutBytes);  // [2][kChunkFloats]
+  PairControl& C = *reinterpret_cast<PairControl*>(sOut + kPairOutBytes + kScaleBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
@@ -157,9 +189,13 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       mbar_init(smem_u32(&C.full[s]), 1);
       mbar_init(smem_u32(&C.empty[s]), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 4; ++b) {
       mbar_init(smem_u32(&C.acc_full[b]), 1);
-      mbar_init(smem_u32(&C.acc_empty[b]), 16);
+      mbar_init(smem_u32(&C.acc_empty[b]), kEpiWarps);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&C.scale_full[b]), 1);
+      mbar_init(smem_u32(&C.scale_empty[b]), kEpiWarps);
     }
     mbar_init(smem_u32(&C.mma_done), 1);
     C.abort_flag = 0;
@@ -170,11 +206,11 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, 912);
     return;
   }
-  if (warp == 9) {
-    tmem_alloc_pair(smem_u32(&C.tmem_base), 2 * kPairAccCols);
+  if (warp == kIssuerWarp) {
+    tmem_alloc_pair(smem_u32(&C.tmem_base), 4 * kPairAccCols);
     tmem_relinquish_pair();
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == kProducerWarp && lane == 0) {
     prefetch_tensormap(&tm_a);
     prefetch_tensormap(&tm_b);
     if (p.tma_out) prefetch_tensormap(&tm_out);
@@ -188,11 +224,13 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   const int64_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int64_t total_tiles = (int64_t)p.m_tiles * p.n_tiles;  // 256 x 256 tiles
 
-  if (warp == 8) {
+  if (warp >= kEpiWarps) {
+  setmaxnreg_dec<kOtherRegs>();
+  if (warp == kProducerWarp) {
     // ------------------------------------------------------------ producer (both CTAs)
-    if (lane == 0) {
+    if (elect_one()) {
       int s = 0, use = 0;
-      int armed[kPairStages] = {};
+      int64_t issued = 0;  // stages
       bool ok = true;
       for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
         int mt, nt;
@@ -204,10 +242,13 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
           }
           const uint32_t full_leader = mapa_shared(smem_u32(&C.full[s]), 0);
           if (leader) mbar_arrive_expect_tx(smem_u32(&C.full[s]), 2 * kPairStageBytes);
-          ++armed[s];
+          ++issued;
           const uint32_t st = base + s * kPairStageBytes;
           tma_load_2d_pair(st, &tm_a, full_leader, kb * kBlockK, mt * 256 + (int)rank * 128);
-          tma_load_2d_pair(st + kPairOpBytes, &tm_b, full_leader, kb * kBlockK, nt * 256 + (int)rank * 128);
+          // of each half's 128 weight rows this CTA holds 64
+          tma_load_2d_pair(st + kPairOpBytes, &tm_b, full_leader, kb * kBlockK, nt * 256 + (int)rank * 64);
+          tma_load_2d_pair(st + kPairOpBytes + kPairHalfBytes, &tm_b, full_leader, kb * kBlockK,
+                           nt * 256 + 128 + (int)rank * 64);
           if (++s == kPairStages) {
             s = 0;
             ++use;
@@ -217,35 +258,34 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       // rank 0's full barriers complete only once both CTAs' bytes have landed
       if (leader)
         for (int st = 0; st < kPairStages; ++st)
-          if (armed[st] > 0) mbar_drain(smem_u32(&C.full[st]), (uint32_t)((armed[st] - 1) & 1));
+          if (issued > st) mbar_drain(smem_u32(&C.full[st]), (uint32_t)(((issued - 1 - st) / kPairStages) & 1));
     }
-  } else if (warp == 9) {
+  } else if (warp == kIssuerWarp) {
     // ------------------------------------------------------------ MMA issuer (rank 0)
-    if (lane == 0 && leader) {
-      constexpr uint32_t idesc = idesc_e4m3_f32(256, 256);
+    if (leader && elect_one()) {
+      constexpr uint32_t idesc = idesc_e4m3_f32(256, 128);
       const uint64_t adesc0 = smem_desc_sw128(base, 16, 1024);
       int s = 0, use = 0, buf = 0;
       uint32_t round = 0;  // how often both accumulators have been filled
       bool ok = true;
       for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
         for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!mbar_wait(smem_u32(&C.acc_empty[buf]), (round & 1u) ^ 1u, abort_flag, p.status, 432) ||
-              !mbar_wait(smem_u32(&C.full[s]), (uint32_t)(use & 1), abort_flag, p.status, 433)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t acc = tmem + buf * kPairAccCols;
+          ok = mbar_wait(smem_u32(&C.full[s]), (uint32_t)(use & 1), abort_flag, p.status, 433);
           const uint64_t sa = adesc0 + (uint64_t)((s * kPairStageBytes) >> 4);
-          const uint64_t sb = sa + (uint64_t)(kPairOpBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kBlockK / 32; ++kk)
-            mma_f8_pair(acc, sa + (uint64_t)(kk * 2), sb + (uint64_t)(kk * 2), idesc, kk > 0 ? 1u : 0u);
-          const uint32_t f = smem_u32(&C.acc_full[buf]), e = smem_u32(&C.empty[s]);
-          tc_commit_pair(mapa_shared(f, 0));
-          tc_commit_pair(mapa_shared(f, 1));
-          tc_commit_pair(mapa_shared(e, 0));
-          tc_commit_pair(mapa_shared(e, 1));
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && mbar_wait(smem_u32(&C.acc_empty[2 * buf + h]), (round & 1u) ^ 1u, abort_flag, p.status, 432);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t sb = sa + (uint64_t)((kPairOpBytes + h * kPairHalfBytes) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < kBlockK / 32; ++kk)
+              mma_f8_pair(tmem + (2 * buf + h) * kPairAccCols, sa + (uint64_t)(kk * 2), sb + (uint64_t)(kk * 2), idesc,
+                          kk > 0 ? 1u : 0u);
+            tc_commit_both(smem_u32(&C.acc_full[2 * buf + h]));
+          }
+          if (!ok) break;
+          tc_commit_both(smem_u32(&C.empty[s]));
           if (++s == kPairStages) {
             s = 0;
             ++use;
@@ -256,92 +296,156 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
           }
         }
       }
-      const uint32_t d = smem_u32(&C.mma_done);  // covers every MMA of the pair
-      tc_commit_pair(mapa_shared(d, 0));
-      tc_commit_pair(mapa_shared(d, 1));
+      tc_commit_both(smem_u32(&C.mma_done));  // covers every MMA of the pair
     }
-  } else {
-    // ------------------------------------------------------------ epilogue (both CTAs)
-    const int quad = warp & 3, half = warp >> 2;
-    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t stage = smem_u32(sOut) + (uint32_t)(warp * kPairOutBox);
-    const uint32_t acc_empty0 = mapa_shared(smem_u32(&C.acc_empty[0]), 0);
-    const uint32_t acc_empty1 = mapa_shared(smem_u32(&C.acc_empty[1]), 0);
-    constexpr int kOutCols = 128 / (int)sizeof(T);  // columns of a staged 128-byte row
+  } else if (warp == kScaleWarp) {
+    // ------------------------------------------------------------ scales (both CTAs)
+    // a_scale[m, kb] * b_scale[n / 128, kb] for the CTA's 128 rows and the tile's two weight
+    // blocks, kChunk k-blocks at a time: lane l serves rows l, l + 32, l + 64 and l + 96.
     int buf = 0;
     uint32_t round = 0;
     bool ok = true;
     for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
       int mt, nt;
       tile_coords(t, p.m_tiles, p.n_tiles, mt, nt);
-      const int64_t m = (int64_t)mt * 256 + rank * 128 + quad * 32 + lane;
-      const int n0 = nt * 256 + half * 128;
-      const bool row_ok = m < p.M && n0 < p.N;
-      // Rows and column blocks outside the matrix hold zeros in TMEM; their scale is 0.
-      const float* sa = p.a_scale + (row_ok ? m * p.a_row_stride : 0);
-      const float* sb = p.b_scale + (row_ok ? (int64_t)(n0 >> 7) * p.k_blocks : 0);
-      uint64_t acc[64];
+      const int64_t m0 = (int64_t)mt * 256 + rank * 128 + lane;
+      const float* sb0 = p.b_scale + (int64_t)(nt * 2) * p.k_blocks;
+      const bool two = nt * 256 + 128 < p.N;
+      for (int k0 = 0; ok && k0 < p.k_blocks; k0 += kChunk) {
+        float a[4][kChunk];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = 0;
-      float scale = row_ok ? __ldg(sa) * __ldg(sb) : 0.f;
-      for (int kb = 0; kb < p.k_blocks; ++kb) {
-        float next = 0.f;
-        if (row_ok && kb + 1 < p.k_blocks) next = __ldg(sa + (kb + 1) * p.a_block_stride) * __ldg(sb + kb + 1);
-        const bool got = mbar_wait(smem_u32(&C.acc_full[buf]), round & 1u, abort_flag, p.status, 434);
-        if (!__all_sync(0xffffffffu, got)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint64_t s2 = f2_pack(scale, scale);
-        const uint32_t col0 = tmem + lane_base + buf * kPairAccCols + half * 128;
+        for (int i = 0; i < 4; ++i) {
+          const int64_t m = m0 + 32 * i;
+          const float* sa = p.a_scale + m * p.a_row_stride;
+          if (m < p.M && p.a_vec && k0 + kChunk <= p.k_blocks) {
+            load8(sa + k0, a[i]);
+          } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tmem_ld32(col0 + 32 * c, r);
-          tmem_wait_ld();
-          if (c == 3) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(buf == 0 ? acc_empty0 : acc_empty1);
+            for (int e = 0; e < kChunk; ++e)
+              a[i][e] = m < p.M && k0 + e < p.k_blocks ? __ldg(sa + (k0 + e) * p.a_block_stride) : 0.f;
           }
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            acc[16 * c + i] = f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s2,
-                                     acc[16 * c + i]);
         }
-        scale = next;
+        const bool got = mbar_wait(smem_u32(&C.scale_empty[buf]), (round & 1u) ^ 1u, abort_flag, p.status, 435);
+        ok = __all_sync(0xffffffffu, got);
+        if (!ok) break;
+        float* dst = sScale + buf * kChunkFloats + lane;
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) {
+          const bool in = k0 + e < p.k_blocks;
+          const float b0 = in ? __ldg(sb0 + k0 + e) : 0.f;
+          const float b1 = in && two ? __ldg(sb0 + p.k_blocks + k0 + e) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            dst[(2 * e) * 128 + 32 * i] = a[i][e] * b0;
+            dst[(2 * e + 1) * 128 + 32 * i] = a[i][e] * b1;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&C.scale_full[buf]));
         if (++buf == 2) {
           buf = 0;
           ++round;
         }
       }
+    }
+  }
+  } else {
+    setmaxnreg_inc<kEpiRegs>();
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int quad = warp & 3, half = warp >> 2;
+    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+    const uint32_t stage = smem_u32(sOut) + (uint32_t)(warp * kPairOutBox);
+    const uint32_t acc_empty = mapa_shared(smem_u32(&C.acc_empty[half]), 0);  // + 16 bytes for buffer 1
+    constexpr int kOutCols = 64 / (int)sizeof(T);  // columns of a staged 64-byte row
+    constexpr int kVec = 16 / (int)sizeof(T);
+    const float* my_scale = sScale + half * 128 + quad * 32 + lane;
+    int buf = 0, chunk = 0;  // accumulator and scale chunk in use
+    uint32_t round = 0, chunk_round = 0;
+    bool ok = true;
+    for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
+      float acc[128];
+#pragma unroll
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        bool got = true;
+        if (kb % kChunk == 0)
+          got = mbar_wait(smem_u32(&C.scale_full[chunk]), chunk_round & 1u, abort_flag, p.status, 436);
+        const float scale = my_scale[chunk * kChunkFloats + (kb % kChunk) * 256];
+        got = got && mbar_wait(smem_u32(&C.acc_full[2 * buf + half]), round & 1u, abort_flag, p.status, 434);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t col0 = tmem + lane_base + (2 * buf + half) * kPairAccCols;
+        // The load of the next 32 columns is in flight while 32 are added.
+        uint32_t r[2][32];
+        tmem_ld32(col0, r[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_ld();
+          if (c < 3) {
+            tmem_ld32(col0 + 32 * (c + 1), r[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 16);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(r[c & 1][i]), scale, acc[32 * c + i]);
+        }
+        if (++buf == 2) {
+          buf = 0;
+          ++round;
+        }
+        if (kb % kChunk == kChunk - 1 || kb == p.k_blocks - 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&C.scale_empty[chunk]));
+          if (++chunk == 2) {
+            chunk = 0;
+            ++chunk_round;
+          }
+        }
+      }
       if (!ok) break;
+      int mt, nt;
+      tile_coords(t, p.m_tiles, p.n_tiles, mt, nt);
+      const int64_t m = (int64_t)mt * 256 + rank * 128 + quad * 32 + lane;
+      const int n0 = nt * 256 + half * 128;
       if (n0 >= p.N) continue;
       // ---------------------------------------------------------- output
+      const bool row_ok = m < p.M;
 #pragma unroll
       for (int g = 0; g < 128 / kOutCols; ++g) {
-        float f[kOutCols];
-#pragma unroll
-        for (int i = 0; i < kOutCols / 2; ++i) f2_unpack(acc[g * (kOutCols / 2) + i], f[2 * i], f[2 * i + 1]);
         const int nc = n0 + g * kOutCols;
-        finish_columns<T, kOutCols>(p, m, row_ok, nc, f);
         if (p.tma_out) {
-          // 16-byte chunk q of staged row r sits at q ^ (r & 7) (128-byte swizzle)
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
+        }
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < 4; ++q) {  // 16 bytes of the row at a time
+          float f[kVec];
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) f[i] = acc[g * kOutCols + q * kVec + i];
+          finish_columns<T>(p, m, row_ok, nc + q * kVec, f);
+          if (p.tma_out) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = sizeof(T) == 2 ? cvt_bf16x2(f[(8 * q + 2 * e) % kOutCols], f[(8 * q + 2 * e + 1) % kOutCols])
-                                    : __float_as_uint(f[(4 * q + e) % kOutCols]);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (uint32_t)(lane * 128 +
-                                                                                            ((q ^ (lane & 7)) * 16))),
+              w[e] = sizeof(T) == 2 ? cvt_bf16x2(f[(2 * e) % kVec], f[(2 * e + 1) % kVec]) : __float_as_uint(f[e]);
+            // chunk q of staged row r sits at q ^ ((r >> 1) & 3) (64-byte swizzle)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             stage + (uint32_t)(lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16))),
                          "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                          : "memory");
+          } else if (row_ok) {
+            T* out = static_cast<T*>(p.out) + m * p.N + nc + q * kVec;
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+              if (nc + q * kVec + i < p.N) out[i] = Elem<T>::from_f(f[i]);
           }
+        }
+        if (p.tma_out) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {  // rows past M and columns past N are clipped by the store
@@ -349,11 +453,6 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
             if (nc < p.N && row0 < p.M) tma_store_2d(&tm_out, stage, nc, (int)row0);
             bulk_commit_group();
           }
-        } else if (row_ok) {
-          T* out = static_cast<T*>(p.out) + m * p.N;
-#pragma unroll
-          for (int i = 0; i < kOutCols; ++i)
-            if (nc + i < p.N) out[nc + i] = Elem<T>::from_f(f[i]);
         }
       }
     }
@@ -364,15 +463,132 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kIssuerWarp) {
     tc_fence_after();
     mbar_drain(smem_u32(&C.mma_done), 0);  // rank 0's MMAs write both CTAs' TMEM
   }
   cluster_sync_all();  // no signal to the peer's shared memory is still in flight
-  if (warp == 9) {
+  if (warp == kIssuerWarp) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, 2 * kPairAccCols);
+    tmem_dealloc_pair(tmem, 4 * kPairAccCols);
   }
+}
+
+// ------------------------------------------------------------------ few rows: plain streaming
+// For up to four rows of A the product is the reading of B once: each thread multiplies its 16
+// bytes of a weight row with its 16 columns of the M rows, which it keeps as fp32, so weights go
+// from global memory to registers with no staging, and no TMEM, barrier or tensor map has to be
+// set up.  A CTA of 8 warps takes kRows weight rows per row group; `kWarps` warps split K (512
+// columns each at a time) and the sums meet in shared memory.
+constexpr int kStreamThreads = 256;
+constexpr int kRows = 8;
+
+__device__ __forceinline__ void e4m3x16_to_float(const uint4& raw, float* f) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w[i >> 1] >> (16 * (i & 1)))));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+
+template <typename T, int M>
+__global__ void __launch_bounds__(kStreamThreads) fp8_gemm_blocks_stream_kernel(const uint8_t* __restrict__ a,
+                                                                                const uint8_t* __restrict__ b,
+                                                                                int k_warps, BlockGemmParams p) {
+  __shared__ float part[kStreamThreads / 32][kRows * M];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows = (int)p.M;  // at most M
+  const int group = warp / k_warps, kw = warp - group * k_warps;
+  const int n0 = (blockIdx.x * (kStreamThreads / 32 / k_warps) + group) * kRows;
+  float acc[kRows * M];  // [row][m]
+#pragma unroll
+  for (int i = 0; i < kRows * M; ++i) acc[i] = 0.f;
+  if (n0 < p.N) {
+    const float* sb = p.b_scale + (int64_t)(n0 >> 7) * p.k_blocks;  // kRows divides 128: one weight block
+    for (int64_t k = (kw * 32 + lane) * 16; k < p.K; k += (int64_t)k_warps * 512) {
+      uint4 w[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        w[r] = __ldg(reinterpret_cast<const uint4*>(b + (int64_t)min(n0 + r, p.N - 1) * p.K + k));
+      const int kb = (int)(k >> 7);
+      const float s = __ldg(sb + kb);
+      float sm[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) sm[m] = s * __ldg(p.a_scale + min(m, rows - 1) * p.a_row_stride + kb * p.a_block_stride);
+      float x[M][16];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+        e4m3x16_to_float(__ldg(reinterpret_cast<const uint4*>(a + (int64_t)min(m, rows - 1) * p.K + k)), x[m]);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        float y[16];
+        e4m3x16_to_float(w[r], y);
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          float d = x[m][0] * y[0];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) d = fmaf(x[m][i], y[i], d);
+          acc[r * M + m] = fmaf(d, sm[m], acc[r * M + m]);
+        }
+      }
+    }
+  }
+  // Sums over the lanes: each step halves the values a lane holds until each holds one or few.
+  int held = kRows * M;
+  int index = 0;  // the first of the values this lane holds
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (held > 1) {
+      held >>= 1;
+      const bool upper = (lane & o) != 0;
+#pragma unroll
+      for (int i = 0; i < kRows * M / 2; ++i) {
+        if (i < held) {
+          const float keep = upper ? acc[i + held] : acc[i];
+          const float give = upper ? acc[i] : acc[i + held];
+          acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      }
+      if (upper) index += held;
+    } else {
+      acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
+    }
+  }
+  // kRows * M is 8, 16 or 32: one value per lane, held by 4, 2 or 1 lanes
+  if (lane % (32 / (kRows * M)) == 0) part[warp][index] = acc[0];
+  __syncthreads();
+  const int groups = kStreamThreads / 32 / k_warps;
+  for (int i = threadIdx.x; i < groups * kRows * M; i += kStreamThreads) {
+    const int g = i / (kRows * M), e = i - g * (kRows * M);
+    const int n = (blockIdx.x * groups + g) * kRows + e / M, m = e % M;
+    if (n >= p.N || m >= rows) continue;
+    float f = 0.f;
+    for (int w = 0; w < k_warps; ++w) f += part[g * k_warps + w][e];
+    if (p.bias != nullptr) f += __ldg(p.bias + n);
+    const int64_t at = (int64_t)m * p.N + n;
+    if (p.residual != nullptr)
+      f = fmaf(p.gate != nullptr ? __ldg(p.gate + n) : 1.f, f, Elem<T>::to_f(static_cast<const T*>(p.residual)[at]));
+    static_cast<T*>(p.out)[at] = Elem<T>::from_f(f);
+  }
+}
+
+template <typename T>
+int launch_stream(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, cudaStream_t s) {
+  int k_warps = 1;
+  while (k_warps < 8 && k_warps * 512 < p.K) k_warps *= 2;
+  const int rows = kRows * (kStreamThreads / 32 / k_warps);
+  const unsigned grid = (unsigned)((p.N + rows - 1) / rows);
+  switch (p.M) {
+    case 1: fp8_gemm_blocks_stream_kernel<T, 1><<<grid, kStreamThreads, 0, s>>>(a, b, k_warps, p); break;
+    case 2: fp8_gemm_blocks_stream_kernel<T, 2><<<grid, kStreamThreads, 0, s>>>(a, b, k_warps, p); break;
+    default: fp8_gemm_blocks_stream_kernel<T, 4><<<grid, kStreamThreads, 0, s>>>(a, b, k_warps, p); break;
+  }
+  SB_CHECK_LAUNCH("sb_fp8_gemm_blocks launch");
+  return SB_OK;
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -391,7 +607,8 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Row-major [rows, cols] as boxes of 128 bytes x box_rows, 128-byte swizzle.
+// Row-major [rows, cols] as boxes of 128 bytes x box_rows (loads, 128-byte swizzle) or 64 bytes x
+// box_rows (stores, 64-byte swizzle).
 int make_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* base, uint64_t cols, uint64_t rows,
              uint32_t box_rows, bool load) {
   EncodeTiledFn encode = encode_fn();
@@ -401,10 +618,10 @@ int make_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* b
   }
   const cuuint64_t dims[2] = {cols, rows};
   const cuuint64_t strides[1] = {cols * (uint64_t)elem};
-  const cuuint32_t box[2] = {(cuuint32_t)(128 / elem), box_rows};
+  const cuuint32_t box[2] = {(cuuint32_t)((load ? 128 : 64) / elem), box_rows};
   const cuuint32_t estr[2] = {1, 1};
   CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B,
+                      load ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                       load ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE,
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -426,7 +643,7 @@ int launch_pair(const uint8_t* a, const uint8_t* b, BlockGemmParams p, cudaStrea
   CUtensorMap ma, mb, mo;
   int rc;
   if ((rc = make_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a, p.K, p.M, 128, true)) != SB_OK) return rc;
-  if ((rc = make_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b, p.K, p.N, 128, true)) != SB_OK) return rc;
+  if ((rc = make_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b, p.K, p.N, 64, true)) != SB_OK) return rc;
   mo = ma;
   if (p.tma_out &&
       (rc = make_map(&mo, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, sizeof(T),
@@ -434,7 +651,7 @@ int launch_pair(const uint8_t* a, const uint8_t* b, BlockGemmParams p, cudaStrea
     return rc;
   p.m_tiles = (int)((p.M + 255) / 256);
   p.n_tiles = (p.N + 255) / 256;
-  const size_t smem = (size_t)kPairStages * kPairStageBytes + kPairOutBytes + sizeof(PairControl);
+  const size_t smem = (size_t)kPairStages * kPairStageBytes + kPairOutBytes + kScaleBytes + sizeof(PairControl);
   cudaError_t err =
       cudaFuncSetAttribute(fp8_gemm_blocks_pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (err != cudaSuccess) return cuda_error(err, "sb_fp8_gemm_blocks: set smem");
@@ -493,7 +710,10 @@ extern "C" int sb_fp8_gemm_blocks(const uint8_t* a, const float* a_scale, int64_
   p.N = N;
   p.K = K;
   p.k_blocks = (K + kBlockK - 1) / kBlockK;
+  p.a_vec = a_block_stride == 1 && a_row_stride % 4 == 0 && (uintptr_t)a_scale % 16 == 0;
   p.tma_out = (int64_t)N * (out_dtype == SB_BF16 ? 2 : 4) % 16 == 0;
   cudaStream_t s = (cudaStream_t)stream;
+  if (M <= 4)
+    return out_dtype == SB_BF16 ? launch_stream<__nv_bfloat16>(a, b, p, s) : launch_stream<float>(a, b, p, s);
   return out_dtype == SB_BF16 ? launch_pair<__nv_bfloat16>(a, b, p, s) : launch_pair<float>(a, b, p, s);
 }

@@ -365,7 +365,7 @@ def assert_gemm(out, want, error):
     assert bool((off <= 0).all()), float(off.max())
 
 
-GEMM_SIZES = [(1, 1, 16), (1, 4096, 4096), (2, 130, 144), (8, 512, 128), (9, 1420, 2000), (17, 392, 4112), (24, 1000, 5376),
+GEMM_SIZES = [(1, 1, 16), (1, 4096, 4096), (2, 130, 144), (2, 4104, 5376), (3, 1000, 512), (3, 77, 10000), (4, 392, 4112), (4, 5, 16), (8, 512, 128), (9, 1420, 2000), (17, 392, 4112), (24, 1000, 5376),
               (33, 129, 256), (64, 2056, 1024), (65, 640, 640), (100, 4096, 400), (128, 257, 16384), (129, 128, 272),
               (200, 3000, 1040), (256, 256, 128), (259, 5376, 1360), (513, 264, 2064), (1000, 392, 4112), (2100, 4104, 912)]
 
@@ -383,7 +383,7 @@ def test_gemm_matches_its_definition(cuda_device, M, N, K, out_dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (5, 131, 400), (40, 264, 1040), (130, 520, 2064), (300, 1001, 272),
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (3, 131, 400), (5, 131, 400), (40, 264, 1040), (130, 520, 2064), (300, 1001, 272),
                                    (2600, 4096, 256)])
 def test_gemm_bias_gate_and_residual(cuda_device, M, N, K, out_dtype):
     a, a_scale, b, b_scale, g = gemm_inputs(M, N, K, cuda_device, M + N + K)
