@@ -631,6 +631,280 @@ int make_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* b
   return SB_OK;
 }
 
+// ------------------------------------------------------------------ some rows: weights as MMA rows
+// A tile is 128 weight rows (the MMA's M) x T rows of A (its N, a multiple of 16 up to 128), so a
+// few rows of A do not fill a 256-row tile with padding.  CTAs are small and several share an SM,
+// which hides each one's set-up and hand-overs behind the others' loads; where the tiles alone do
+// not fill the GPU, the CTAs of a cluster split K and add their sums, in rank order, through
+// distributed shared memory.  Thread = weight row: the scale of accumulator column j is
+// a_scale[row j] * b_scale, read from shared memory by all lanes at once.
+//   warps 0 .. EW-1 epilogue (EW 4: all columns; EW 8: warps 4-7 take the upper half), then the
+//   TMA producer, the MMA issuer and the scale warp.
+constexpr int kSwapMaxStages = 4;
+constexpr int kSwapRing = 4;  // TMEM buffers at most
+
+struct __align__(8) SwapControl {
+  uint64_t full[kSwapMaxStages], empty[kSwapMaxStages];
+  uint64_t acc_full[kSwapRing], acc_empty[kSwapRing];
+  uint64_t scale_full[2], scale_empty[2];
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct SwapShape {
+  int tokens;      // T: rows of A per tile
+  int m_tiles;
+  int splits;      // CTAs of a cluster
+  int stages, ring;
+  uint32_t acc_stride;  // TMEM columns per buffer; ring * acc_stride are allocated
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// One output value from its sum.
+template <typename T>
+__device__ __forceinline__ void finish_value(const BlockGemmParams& p, int64_t m, int n, float f) {
+  if (p.bias != nullptr) f += __ldg(p.bias + n);
+  const int64_t at = m * p.N + n;
+  if (p.residual != nullptr)
+    f = fmaf(p.gate != nullptr ? __ldg(p.gate + n) : 1.f, f, Elem<T>::to_f(static_cast<const T*>(p.residual)[at]));
+  static_cast<T*>(p.out)[at] = Elem<T>::from_f(f);
+}
+
+template <typename T, int EW, int CW>
+__global__ void __launch_bounds__(32 * (EW + 3), 2)
+fp8_gemm_blocks_swap_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                            BlockGemmParams p, SwapShape q) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const bool aligned = (smem_u32(smem) & 1023u) == 0u;  // alike in every CTA
+  const int tokens = q.tokens;
+  const int stage_bytes = kPairOpBytes + tokens * kBlockK;
+  float* sScale = reinterpret_cast<float*>(smem + q.stages * stage_bytes);  // [2][kChunk][tokens]
+  SwapControl& C = *reinterpret_cast<SwapControl*>(sScale + 2 * kChunk * tokens);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % q.splits;
+  const int tile = blockIdx.x / q.splits;
+  const int mt = tile % q.m_tiles, nt = tile / q.m_tiles;  // tiles of one weight panel run together
+  const int kb0 = (int)((int64_t)p.k_blocks * rank / q.splits);
+  const int kb1 = (int)((int64_t)p.k_blocks * (rank + 1) / q.splits);
+  if (!aligned) {
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, 913);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSwapMaxStages; ++s) {
+      mbar_init(smem_u32(&C.full[s]), 1);
+      mbar_init(smem_u32(&C.empty[s]), 1);
+    }
+    for (int b = 0; b < kSwapRing; ++b) {
+      mbar_init(smem_u32(&C.acc_full[b]), 1);
+      mbar_init(smem_u32(&C.acc_empty[b]), EW);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&C.scale_full[b]), 1);
+      mbar_init(smem_u32(&C.scale_empty[b]), EW);
+    }
+    mbar_init(smem_u32(&C.mma_done), 1);
+    C.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == EW + 1) {
+    tmem_alloc(smem_u32(&C.tmem_base), q.ring * q.acc_stride);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = C.tmem_base;
+  volatile int* abort_flag = &C.abort_flag;
+  const uint32_t base = smem_u32(smem);
+
+  float acc[CW];
+#pragma unroll
+  for (int i = 0; i < CW; ++i) acc[i] = 0.f;
+  const int quad = warp & 3;
+  const int col0 = EW == 8 && warp >= 4 ? (tokens + 31) / 32 * 16 : 0;
+  const int cols = EW == 8 ? (warp >= 4 ? tokens - col0 : (tokens + 31) / 32 * 16) : tokens;
+
+  if (warp == EW) {
+    // ------------------------------------------------------------ producer
+    if (elect_one()) {
+      int s = 0;
+      uint32_t use = 0;
+      int issued = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&C.empty[s]), (use & 1u) ^ 1u, abort_flag, p.status, 441)) break;
+        const uint32_t st = base + s * stage_bytes, full = smem_u32(&C.full[s]);
+        mbar_arrive_expect_tx(full, stage_bytes);
+        tma_load_2d(st, &tm_b, full, kb * kBlockK, nt * 128);
+        tma_load_2d(st + kPairOpBytes, &tm_a, full, kb * kBlockK, mt * tokens);
+        ++issued;
+        if (++s == q.stages) {
+          s = 0;
+          ++use;
+        }
+      }
+      for (int st = 0; st < q.stages; ++st)
+        if (issued > st) mbar_drain(smem_u32(&C.full[st]), (uint32_t)(((issued - 1 - st) / q.stages) & 1));
+    }
+  } else if (warp == EW + 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      const uint32_t idesc = idesc_e4m3_f32(128, tokens);
+      const uint64_t desc0 = smem_desc_sw128(base, 16, 1024);
+      int s = 0, buf = 0;
+      uint32_t use = 0, round = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&C.full[s]), use & 1u, abort_flag, p.status, 442) ||
+            !mbar_wait(smem_u32(&C.acc_empty[buf]), (round & 1u) ^ 1u, abort_flag, p.status, 443))
+          break;
+        tc_fence_after();
+        const uint64_t dw = desc0 + (uint64_t)((s * stage_bytes) >> 4);
+        const uint64_t dx = dw + (uint64_t)(kPairOpBytes >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kBlockK / 32; ++kk)
+          mma_f8(tmem + buf * q.acc_stride, dw + (uint64_t)(kk * 2), dx + (uint64_t)(kk * 2), idesc, kk > 0 ? 1u : 0u);
+        tc_commit(smem_u32(&C.acc_full[buf]));
+        tc_commit(smem_u32(&C.empty[s]));
+        if (++s == q.stages) {
+          s = 0;
+          ++use;
+        }
+        if (++buf == q.ring) {
+          buf = 0;
+          ++round;
+        }
+      }
+      tc_commit(smem_u32(&C.mma_done));
+    }
+  } else if (warp == EW + 2) {
+    // ------------------------------------------------------------ scales
+    const float* sb = p.b_scale + (int64_t)nt * p.k_blocks;
+    int buf = 0;
+    uint32_t round = 0;
+    for (int k0 = kb0; k0 < kb1; k0 += kChunk) {
+      const bool got = mbar_wait(smem_u32(&C.scale_empty[buf]), (round & 1u) ^ 1u, abort_flag, p.status, 444);
+      if (!__all_sync(0xffffffffu, got)) break;
+      for (int j = lane; j < tokens; j += 32) {
+        const int64_t m = (int64_t)mt * tokens + j;
+        const float* sa = p.a_scale + m * p.a_row_stride;
+        float v[kChunk];
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e)
+          v[e] = m < p.M && k0 + e < kb1 ? __ldg(sa + (k0 + e) * p.a_block_stride) * __ldg(sb + k0 + e) : 0.f;
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) sScale[(buf * kChunk + e) * tokens + j] = v[e];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&C.scale_full[buf]));
+      if (++buf == 2) {
+        buf = 0;
+        ++round;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+    int buf = 0, chunk = 0;
+    uint32_t round = 0, chunk_round = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int e = (kb - kb0) % kChunk;
+      bool got = true;
+      if (e == 0) got = mbar_wait(smem_u32(&C.scale_full[chunk]), chunk_round & 1u, abort_flag, p.status, 445);
+      got = got && mbar_wait(smem_u32(&C.acc_full[buf]), round & 1u, abort_flag, p.status, 446);
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc_fence_after();
+      const float4* scale = reinterpret_cast<const float4*>(sScale + (chunk * kChunk + e) * tokens + col0);
+      const uint32_t src = tmem + lane_base + buf * q.acc_stride + col0;
+#pragma unroll
+      for (int c = 0; c < CW; c += 16) {
+        if (c < cols) {
+          uint32_t r[16];
+          tmem_ld16(src + c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 s = scale[c / 4 + i];
+            acc[c + 4 * i + 0] = fmaf(__uint_as_float(r[4 * i + 0]), s.x, acc[c + 4 * i + 0]);
+            acc[c + 4 * i + 1] = fmaf(__uint_as_float(r[4 * i + 1]), s.y, acc[c + 4 * i + 1]);
+            acc[c + 4 * i + 2] = fmaf(__uint_as_float(r[4 * i + 2]), s.z, acc[c + 4 * i + 2]);
+            acc[c + 4 * i + 3] = fmaf(__uint_as_float(r[4 * i + 3]), s.w, acc[c + 4 * i + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&C.acc_empty[buf]));
+      if (++buf == q.ring) {
+        buf = 0;
+        ++round;
+      }
+      if (e == kChunk - 1 || kb == kb1 - 1) {
+        if (lane == 0) mbar_arrive(smem_u32(&C.scale_empty[chunk]));
+        if (++chunk == 2) {
+          chunk = 0;
+          ++chunk_round;
+        }
+      }
+    }
+    const int n = nt * 128 + quad * 32 + lane;
+    if (q.splits == 1) {
+      if (n < p.N) {
+#pragma unroll
+        for (int j = 0; j < CW; ++j) {
+          const int64_t m = (int64_t)mt * tokens + col0 + j;
+          if (j < cols && m < p.M) finish_value<T>(p, m, n, acc[j]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == EW + 1) {
+    tc_fence_after();
+    mbar_drain(smem_u32(&C.mma_done), 0);
+    tmem_dealloc(tmem, q.ring * q.acc_stride);
+  }
+  if (q.splits > 1) {
+    // Every stage has been read: the stages hold this CTA's sums as [column][weight row].
+    __syncthreads();
+    float* part = reinterpret_cast<float*>(smem);
+    if (warp < EW) {
+#pragma unroll
+      for (int j = 0; j < CW; ++j)
+        if (j < cols) part[(col0 + j) * 128 + quad * 32 + lane] = acc[j];
+    }
+    cluster_sync_all();
+    const int per = tokens / q.splits;  // columns this CTA finishes; splits divides 16
+    for (int i = threadIdx.x; i < per * 128; i += 32 * (EW + 3)) {
+      const int j = rank * per + i / 128, row = i % 128;
+      float f = 0.f;
+      for (int r = 0; r < q.splits; ++r)
+        f += __uint_as_float(ld_shared_cluster_u32(mapa_shared(smem_u32(part + j * 128 + row), r)));
+      const int64_t m = (int64_t)mt * tokens + j;
+      const int n = nt * 128 + row;
+      if (m < p.M && n < p.N) finish_value<T>(p, m, n, f);
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its sums
+  }
+}
+
 int sm_count() {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -674,6 +948,53 @@ int launch_pair(const uint8_t* a, const uint8_t* b, BlockGemmParams p, cudaStrea
   return SB_OK;
 }
 
+template <typename T, int EW, int CW>
+int launch_swap(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, SwapShape q, cudaStream_t s) {
+  CUtensorMap ma, mb;
+  int rc;
+  if ((rc = make_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a, p.K, p.M, q.tokens, true)) != SB_OK) return rc;
+  if ((rc = make_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b, p.K, p.N, 128, true)) != SB_OK) return rc;
+  const size_t smem = (size_t)q.stages * (kPairOpBytes + q.tokens * kBlockK) + (size_t)2 * kChunk * q.tokens * 4 +
+                      sizeof(SwapControl);
+  auto kernel = fp8_gemm_blocks_swap_kernel<T, EW, CW>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (err != cudaSuccess) return cuda_error(err, "sb_fp8_gemm_blocks: set smem");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((int64_t)q.m_tiles * ((p.N + 127) / 128) * q.splits), 1, 1);
+  cfg.blockDim = dim3(32 * (EW + 3), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = q.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, kernel, ma, mb, p, q);
+  if (err != cudaSuccess) return cuda_error(err, "sb_fp8_gemm_blocks: cluster launch");
+  SB_CHECK_LAUNCH("sb_fp8_gemm_blocks launch");
+  return SB_OK;
+}
+
+template <typename T>
+int dispatch_swap(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, cudaStream_t s) {
+  SwapShape q{};
+  q.m_tiles = (int)((p.M + 127) / 128);
+  q.tokens = (int)((p.M + q.m_tiles - 1) / q.m_tiles + 15) / 16 * 16;
+  const int64_t tiles = (int64_t)q.m_tiles * ((p.N + 127) / 128);
+  // Split K until there are two CTAs per SM, each with at least four k-blocks.
+  q.splits = 1;
+  while (q.splits < 8 && tiles * q.splits < 2 * sm_count() && p.k_blocks >= 8 * q.splits) q.splits *= 2;
+  q.stages = q.tokens <= 16 ? 4 : 3;
+  q.acc_stride = q.tokens <= 32 ? 32 : q.tokens <= 64 ? 64 : 128;
+  q.ring = q.tokens <= 32 ? 4 : 2;
+  if (q.tokens <= 16) return launch_swap<T, 4, 16>(a, b, p, q, s);
+  if (q.tokens <= 32) return launch_swap<T, 4, 32>(a, b, p, q, s);
+  if (q.tokens <= 64) return launch_swap<T, 4, 64>(a, b, p, q, s);
+  return launch_swap<T, 8, 64>(a, b, p, q, s);
+}
+
 }  // namespace
 }  // namespace sb
 
@@ -715,5 +1036,7 @@ extern "C" int sb_fp8_gemm_blocks(const uint8_t* a, const float* a_scale, int64_
   cudaStream_t s = (cudaStream_t)stream;
   if (M <= 4)
     return out_dtype == SB_BF16 ? launch_stream<__nv_bfloat16>(a, b, p, s) : launch_stream<float>(a, b, p, s);
+  if (M <= 1024)
+    return out_dtype == SB_BF16 ? dispatch_swap<__nv_bfloat16>(a, b, p, s) : dispatch_swap<float>(a, b, p, s);
   return out_dtype == SB_BF16 ? launch_pair<__nv_bfloat16>(a, b, p, s) : launch_pair<float>(a, b, p, s);
 }

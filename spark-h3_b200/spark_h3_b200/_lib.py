@@ -120,3 +120,15 @@ def call(name: str, *args) -> int:
     status = getattr(load(), name)(*args)
     check(status, name)
     return status
+
+
+_bound = {}
+
+
+def bound(name: str):
+    """The entry point itself, looked up once: for wrappers whose host time is a good part of the
+    kernel's.  The caller checks a negative status with check()."""
+    fn = _bound.get(name)
+    if fn is None:
+        fn = _bound[name] = getattr(load(), name)
+    return fn

@@ -113,8 +113,8 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _strided_rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
-    """x [M, C] with unit-stride, non-overlapping rows (copied when it has none) and the
+def _strided_rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int]:
+    """x [M, C] with unit-stride, non-overlapping rows (copied when it has none), M, C and the
     distance between its rows."""
     if x.dim() != 2:
         raise ValueError(f"{name} must be [M, K], got {tuple(x.shape)}")
@@ -123,9 +123,12 @@ def _strided_rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
     M, C = x.shape
     if C == 0:
         raise ValueError(f"{name} has no columns")
-    if x.stride(1) != 1 or (M > 1 and x.stride(0) < C):
-        x = x.contiguous()
-    return x, x.stride(0) if M > 1 else C
+    if x.is_contiguous():
+        return x, M, C, C
+    stride, unit = x.stride()
+    if unit != 1 or (M > 1 and stride < C):
+        x, stride = x.contiguous(), C
+    return x, M, C, stride if M > 1 else C
 
 
 def _same_device(device: torch.device, **tensors) -> None:
@@ -135,26 +138,32 @@ def _same_device(device: torch.device, **tensors) -> None:
 
 
 def _call_on(device: torch.device, name: str, *args) -> None:
-    """The C-ABI call with `device` current, on its current stream."""
-    stream = _stream(device)
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, stream)
+    """The C-ABI call with `device` current, on its current stream.  These operators take a few
+    microseconds on a few rows, so the host side keeps to the cheapest forms of both queries."""
+    index = device.index
+    fn = _lib.bound(name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, stream)
+            status = fn(*args, stream)
+    if status < 0:
+        _lib.check(status, name)
 
 
 def _quantize_blocks(entry: str, x: torch.Tensor, halves: int):
-    x, stride = _strided_rows(x, "x")
+    x, M, K, stride = _strided_rows(x, "x")
     dtype = _dtype_code(x)
-    M, K = x.shape
-    if K % halves:
-        raise ValueError(f"a [M, 2K] projection output is expected, got {tuple(x.shape)}")
-    K //= halves
-    y = torch.empty((M, K), device=x.device, dtype=FP8_DTYPE)
-    scale = torch.empty((M, _blocks(K)), device=x.device, dtype=torch.float32)
+    if halves != 1:
+        if K % halves:
+            raise ValueError(f"a [M, 2K] projection output is expected, got {tuple(x.shape)}")
+        K //= halves
+    device = x.device
+    y = torch.empty(M, K, device=device, dtype=FP8_DTYPE)
+    scale = torch.empty(M, -(-K // BLOCK), device=device, dtype=torch.float32)
     if M > 0:
-        _call_on(x.device, entry, x.data_ptr(), stride, dtype, M, K, y.data_ptr(), scale.data_ptr())
+        _call_on(device, entry, x.data_ptr(), stride, dtype, M, K, y.data_ptr(), scale.data_ptr())
     return y, scale
 
 
@@ -179,12 +188,14 @@ def _sample_vector(v: torch.Tensor | None, name: str, M: int, C: int, samples: i
     """A vector [C] or one per sample [S, C] as (fp32 tensor, stride between samples, S)."""
     if v is None:
         return None, 0, samples
-    if v.dim() not in (1, 2) or v.shape[-1] != C:
+    dims = v.dim()
+    if dims not in (1, 2) or v.shape[-1] != C:
         raise ValueError(f"{name} must be [{C}] or [samples, {C}], got {tuple(v.shape)}")
-    v = v.float()
-    if v.stride(-1) != 1 and C > 1:
+    if v.dtype != torch.float32:
+        v = v.float()
+    if not v.is_contiguous() and v.stride(-1) != 1:
         v = v.contiguous()
-    if v.dim() == 1 or v.shape[0] == 1:
+    if dims == 1 or v.shape[0] == 1:
         return v, 0, samples
     S = v.shape[0]
     if S == 0 or M % S or (samples not in (1, S)):
@@ -203,9 +214,8 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
     or [M, 1] (for fp8_gemm); s in x's dtype, written to `out` when given (which may be the
     residual itself: the residual stream updated in place), or None without a residual.  The
     norm works on the unrounded fp32 sum."""
-    x, x_stride = _strided_rows(x, "x")
+    x, M, C, x_stride = _strided_rows(x, "x")
     device, dtype = x.device, _dtype_code(x)
-    M, C = x.shape
     r_stride = 0
     if residual is None:
         if gate is not None or out is not None:
@@ -214,9 +224,9 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"the residual must match x: {tuple(residual.shape)} {residual.dtype}, "
                              f"not {tuple(x.shape)} {x.dtype}")
-        residual, r_stride = _strided_rows(residual, "residual")
+        residual, _, _, r_stride = _strided_rows(residual, "residual")
         if out is None:
-            out = torch.empty((M, C), device=device, dtype=x.dtype)
+            out = torch.empty(M, C, device=device, dtype=x.dtype)
         elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {tuple(x.shape)} {x.dtype}")
     _same_device(device, residual=residual, weight=weight, gate=gate, shift=shift, out=out)
@@ -224,8 +234,8 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
     gate, g_stride, samples = _sample_vector(gate, "gate", M, C, samples)
     weight, w_stride, samples = _sample_vector(weight, "weight", M, C, samples)
     shift, s_stride, samples = _sample_vector(shift, "shift", M, C, samples)
-    y = torch.empty((M, C), device=device, dtype=FP8_DTYPE)
-    scale = torch.empty((M, _blocks(C) if blocks else 1), device=device, dtype=torch.float32)
+    y = torch.empty(M, C, device=device, dtype=FP8_DTYPE)
+    scale = torch.empty(M, _blocks(C) if blocks else 1, device=device, dtype=torch.float32)
     if M > 0:
         _call_on(device, "sb_fp8_add_rms_norm_quantize", x.data_ptr(), x_stride, _ptr(residual), r_stride, _ptr(gate),
                  g_stride, _ptr(weight), w_stride, _ptr(shift), s_stride, dtype, M, C, M // samples, eps, int(blocks),
@@ -261,7 +271,7 @@ def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Ten
     elif out_dtype is None:
         out_dtype = torch.bfloat16
     if out is None:
-        out = torch.empty((M, N), device=device, dtype=out_dtype)
+        out = torch.empty(M, N, device=device, dtype=out_dtype)
     elif out.shape != (M, N) or out.dtype != out_dtype or not out.is_contiguous():
         raise ValueError(f"out must be contiguous [{M}, {N}] {out_dtype}")
     code = _dtype_code(out)
