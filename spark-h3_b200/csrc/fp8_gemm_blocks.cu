@@ -51,20 +51,21 @@ struct BlockGemmParams {
 // next first one (the commit, the read-back, the arrival at rank 0) against the time of the
 // three halves between.  Halves shorten both the MMAs and the read-back in that loop.
 //   full[s]      rank 0 only: armed for both CTAs' bytes of a stage
-//   empty[s]     both CTAs: the MMA's commit releases the stage
+//   empty[s]     both CTAs: the commits of both halves' MMAs release the stage
 //   acc_full[a]  both CTAs, a = 2 * buffer + half: the commit after a half's four MMAs
 //   acc_empty[a] rank 0 only: one arrival per epilogue warp of that half in both CTAs (8)
 //   scale_full[c], scale_empty[c]  per CTA: a chunk of 8 k-blocks' scales, from the scale warp to
 //                the epilogue warps
-//   mma_done     both CTAs: final commit, waited before TMEM is freed
+//   mma_done     both CTAs: the final commits of both issuers, waited before TMEM is freed
+// Each half has its own issuing warp: one waiting for its half's read-back does not hold up the other.
 // Eight epilogue warps per CTA: warp w reads TMEM lanes 32 (w % 4) .. (its 32 rows) of half w / 4
 // (one weight block), so a k-block has ONE scale per thread, a_scale * b_scale.  The 128
 // accumulators of a thread stay in registers for the whole tile (setmaxnreg moves registers of
 // the other four warps to these eight).
 constexpr int kEpiWarps = 8;
 constexpr int kEpiThreads = 32 * kEpiWarps;
-constexpr int kProducerWarp = kEpiWarps, kIssuerWarp = kEpiWarps + 1, kScaleWarp = kEpiWarps + 2;
-constexpr int kPairThreads = kEpiThreads + 128;  // one warp idle
+constexpr int kProducerWarp = kEpiWarps, kScaleWarp = kEpiWarps + 1, kIssuerWarp = kEpiWarps + 2;  // and + 3
+constexpr int kPairThreads = kEpiThreads + 128;
 constexpr int kLaunchRegs = 168, kEpiRegs = 208, kOtherRegs = 88;  // per thread
 static_assert(kEpiRegs * kEpiThreads + kOtherRegs * 128 == kLaunchRegs * kPairThreads,
               "setmaxnreg redistributes exactly what the CTA was launched with");
@@ -171,6 +172,13 @@ __device__ __forceinline__ void finish_columns(const BlockGemmParams& p, int64_t
   }
 }
 
+// The bounded wait of a converged warp: true once the phase is complete.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                          int site) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kPairThreads, 1)
 fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
@@ -187,7 +195,7 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   if (aligned && threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(smem_u32(&C.full[s]), 1);
-      mbar_init(smem_u32(&C.empty[s]), 1);
+      mbar_init(smem_u32(&C.empty[s]), 2);
     }
     for (int b = 0; b < 4; ++b) {
       mbar_init(smem_u32(&C.acc_full[b]), 1);
@@ -197,7 +205,7 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       mbar_init(smem_u32(&C.scale_full[b]), 1);
       mbar_init(smem_u32(&C.scale_empty[b]), kEpiWarps);
     }
-    mbar_init(smem_u32(&C.mma_done), 1);
+    mbar_init(smem_u32(&C.mma_done), 2);
     C.abort_flag = 0;
     fence_barrier_init();
   }
@@ -225,130 +233,129 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   const int64_t total_tiles = (int64_t)p.m_tiles * p.n_tiles;  // 256 x 256 tiles
 
   if (warp >= kEpiWarps) {
-  setmaxnreg_dec<kOtherRegs>();
-  if (warp == kProducerWarp) {
-    // ------------------------------------------------------------ producer (both CTAs)
-    if (elect_one()) {
-      int s = 0, use = 0;
-      int64_t issued = 0;  // stages
+    setmaxnreg_dec<kOtherRegs>();
+    if (warp == kProducerWarp) {
+      // ------------------------------------------------------------ producer (both CTAs)
+      if (elect_one()) {
+        int s = 0, use = 0;
+        int64_t issued = 0;  // stages
+        bool ok = true;
+        for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
+          int mt, nt;
+          tile_coords(t, p.m_tiles, p.n_tiles, mt, nt);
+          for (int kb = 0; kb < p.k_blocks; ++kb) {
+            if (!mbar_wait(smem_u32(&C.empty[s]), (uint32_t)((use & 1) ^ 1), abort_flag, p.status, 431)) {
+              ok = false;
+              break;
+            }
+            const uint32_t full_leader = mapa_shared(smem_u32(&C.full[s]), 0);
+            if (leader) mbar_arrive_expect_tx(smem_u32(&C.full[s]), 2 * kPairStageBytes);
+            ++issued;
+            const uint32_t st = base + s * kPairStageBytes;
+            tma_load_2d_pair(st, &tm_a, full_leader, kb * kBlockK, mt * 256 + (int)rank * 128);
+            // of each half's 128 weight rows this CTA holds 64
+            tma_load_2d_pair(st + kPairOpBytes, &tm_b, full_leader, kb * kBlockK, nt * 256 + (int)rank * 64);
+            tma_load_2d_pair(st + kPairOpBytes + kPairHalfBytes, &tm_b, full_leader, kb * kBlockK,
+                             nt * 256 + 128 + (int)rank * 64);
+            if (++s == kPairStages) {
+              s = 0;
+              ++use;
+            }
+          }
+        }
+        // rank 0's full barriers complete only once both CTAs' bytes have landed
+        if (leader)
+          for (int st = 0; st < kPairStages; ++st)
+            if (issued > st) mbar_drain(smem_u32(&C.full[st]), (uint32_t)(((issued - 1 - st) / kPairStages) & 1));
+      }
+    } else if (warp >= kIssuerWarp) {
+      // ------------------------------------------------------------ MMA issuers (rank 0), one per half
+      const int h = warp - kIssuerWarp;
+      if (leader && elect_one()) {
+        constexpr uint32_t idesc = idesc_e4m3_f32(256, 128);
+        const uint64_t adesc0 = smem_desc_sw128(base, 16, 1024);
+        const uint64_t bdesc0 = adesc0 + (uint64_t)((kPairOpBytes + h * kPairHalfBytes) >> 4);
+        int s = 0, buf = 0;
+        uint32_t use = 0, round = 0;  // how often all stages / both accumulators have been filled
+        bool ok = true;
+        for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
+          for (int kb = 0; kb < p.k_blocks; ++kb) {
+            if (!mbar_wait(smem_u32(&C.full[s]), use & 1u, abort_flag, p.status, 433) ||
+                !mbar_wait(smem_u32(&C.acc_empty[2 * buf + h]), (round & 1u) ^ 1u, abort_flag, p.status, 432)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t off = (uint64_t)((s * kPairStageBytes) >> 4);
+  #pragma unroll
+            for (int kk = 0; kk < kBlockK / 32; ++kk)
+              mma_f8_pair(tmem + (2 * buf + h) * kPairAccCols, adesc0 + off + (uint64_t)(kk * 2),
+                          bdesc0 + off + (uint64_t)(kk * 2), idesc, kk > 0 ? 1u : 0u);
+            tc_commit_both(smem_u32(&C.acc_full[2 * buf + h]));
+            tc_commit_both(smem_u32(&C.empty[s]));
+            if (++s == kPairStages) {
+              s = 0;
+              ++use;
+            }
+            if (++buf == 2) {
+              buf = 0;
+              ++round;
+            }
+          }
+        }
+        tc_commit_both(smem_u32(&C.mma_done));  // covers this warp's MMAs
+      }
+    } else if (warp == kScaleWarp) {
+      // ------------------------------------------------------------ scales (both CTAs)
+      // a_scale[m, kb] * b_scale[n / 128, kb] for the CTA's 128 rows and the tile's two weight
+      // blocks, kChunk k-blocks at a time: lane l serves rows l, l + 32, l + 64 and l + 96.
+      int buf = 0;
+      uint32_t round = 0;
       bool ok = true;
       for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
         int mt, nt;
         tile_coords(t, p.m_tiles, p.n_tiles, mt, nt);
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!mbar_wait(smem_u32(&C.empty[s]), (uint32_t)((use & 1) ^ 1), abort_flag, p.status, 431)) {
-            ok = false;
-            break;
+        const int64_t m0 = (int64_t)mt * 256 + rank * 128 + lane;
+        const float* sb0 = p.b_scale + (int64_t)(nt * 2) * p.k_blocks;
+        const bool two = nt * 256 + 128 < p.N;
+        for (int k0 = 0; ok && k0 < p.k_blocks; k0 += kChunk) {
+          float a[4][kChunk];
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t m = m0 + 32 * i;
+            const float* sa = p.a_scale + m * p.a_row_stride;
+            if (m < p.M && p.a_vec && k0 + kChunk <= p.k_blocks) {
+              load8(sa + k0, a[i]);
+            } else {
+  #pragma unroll
+              for (int e = 0; e < kChunk; ++e)
+                a[i][e] = m < p.M && k0 + e < p.k_blocks ? __ldg(sa + (k0 + e) * p.a_block_stride) : 0.f;
+            }
           }
-          const uint32_t full_leader = mapa_shared(smem_u32(&C.full[s]), 0);
-          if (leader) mbar_arrive_expect_tx(smem_u32(&C.full[s]), 2 * kPairStageBytes);
-          ++issued;
-          const uint32_t st = base + s * kPairStageBytes;
-          tma_load_2d_pair(st, &tm_a, full_leader, kb * kBlockK, mt * 256 + (int)rank * 128);
-          // of each half's 128 weight rows this CTA holds 64
-          tma_load_2d_pair(st + kPairOpBytes, &tm_b, full_leader, kb * kBlockK, nt * 256 + (int)rank * 64);
-          tma_load_2d_pair(st + kPairOpBytes + kPairHalfBytes, &tm_b, full_leader, kb * kBlockK,
-                           nt * 256 + 128 + (int)rank * 64);
-          if (++s == kPairStages) {
-            s = 0;
-            ++use;
-          }
-        }
-      }
-      // rank 0's full barriers complete only once both CTAs' bytes have landed
-      if (leader)
-        for (int st = 0; st < kPairStages; ++st)
-          if (issued > st) mbar_drain(smem_u32(&C.full[st]), (uint32_t)(((issued - 1 - st) / kPairStages) & 1));
-    }
-  } else if (warp == kIssuerWarp) {
-    // ------------------------------------------------------------ MMA issuer (rank 0)
-    if (leader && elect_one()) {
-      constexpr uint32_t idesc = idesc_e4m3_f32(256, 128);
-      const uint64_t adesc0 = smem_desc_sw128(base, 16, 1024);
-      int s = 0, use = 0, buf = 0;
-      uint32_t round = 0;  // how often both accumulators have been filled
-      bool ok = true;
-      for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          ok = mbar_wait(smem_u32(&C.full[s]), (uint32_t)(use & 1), abort_flag, p.status, 433);
-          const uint64_t sa = adesc0 + (uint64_t)((s * kPairStageBytes) >> 4);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ok = ok && mbar_wait(smem_u32(&C.acc_empty[2 * buf + h]), (round & 1u) ^ 1u, abort_flag, p.status, 432);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t sb = sa + (uint64_t)((kPairOpBytes + h * kPairHalfBytes) >> 4);
-#pragma unroll
-            for (int kk = 0; kk < kBlockK / 32; ++kk)
-              mma_f8_pair(tmem + (2 * buf + h) * kPairAccCols, sa + (uint64_t)(kk * 2), sb + (uint64_t)(kk * 2), idesc,
-                          kk > 0 ? 1u : 0u);
-            tc_commit_both(smem_u32(&C.acc_full[2 * buf + h]));
-          }
+          const bool got = mbar_wait(smem_u32(&C.scale_empty[buf]), (round & 1u) ^ 1u, abort_flag, p.status, 435);
+          ok = __all_sync(0xffffffffu, got);
           if (!ok) break;
-          tc_commit_both(smem_u32(&C.empty[s]));
-          if (++s == kPairStages) {
-            s = 0;
-            ++use;
+          float* dst = sScale + buf * kChunkFloats + lane;
+  #pragma unroll
+          for (int e = 0; e < kChunk; ++e) {
+            const bool in = k0 + e < p.k_blocks;
+            const float b0 = in ? __ldg(sb0 + k0 + e) : 0.f;
+            const float b1 = in && two ? __ldg(sb0 + p.k_blocks + k0 + e) : 0.f;
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              dst[(2 * e) * 128 + 32 * i] = a[i][e] * b0;
+              dst[(2 * e + 1) * 128 + 32 * i] = a[i][e] * b1;
+            }
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&C.scale_full[buf]));
           if (++buf == 2) {
             buf = 0;
             ++round;
           }
         }
       }
-      tc_commit_both(smem_u32(&C.mma_done));  // covers every MMA of the pair
     }
-  } else if (warp == kScaleWarp) {
-    // ------------------------------------------------------------ scales (both CTAs)
-    // a_scale[m, kb] * b_scale[n / 128, kb] for the CTA's 128 rows and the tile's two weight
-    // blocks, kChunk k-blocks at a time: lane l serves rows l, l + 32, l + 64 and l + 96.
-    int buf = 0;
-    uint32_t round = 0;
-    bool ok = true;
-    for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
-      int mt, nt;
-      tile_coords(t, p.m_tiles, p.n_tiles, mt, nt);
-      const int64_t m0 = (int64_t)mt * 256 + rank * 128 + lane;
-      const float* sb0 = p.b_scale + (int64_t)(nt * 2) * p.k_blocks;
-      const bool two = nt * 256 + 128 < p.N;
-      for (int k0 = 0; ok && k0 < p.k_blocks; k0 += kChunk) {
-        float a[4][kChunk];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t m = m0 + 32 * i;
-          const float* sa = p.a_scale + m * p.a_row_stride;
-          if (m < p.M && p.a_vec && k0 + kChunk <= p.k_blocks) {
-            load8(sa + k0, a[i]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < kChunk; ++e)
-              a[i][e] = m < p.M && k0 + e < p.k_blocks ? __ldg(sa + (k0 + e) * p.a_block_stride) : 0.f;
-          }
-        }
-        const bool got = mbar_wait(smem_u32(&C.scale_empty[buf]), (round & 1u) ^ 1u, abort_flag, p.status, 435);
-        ok = __all_sync(0xffffffffu, got);
-        if (!ok) break;
-        float* dst = sScale + buf * kChunkFloats + lane;
-#pragma unroll
-        for (int e = 0; e < kChunk; ++e) {
-          const bool in = k0 + e < p.k_blocks;
-          const float b0 = in ? __ldg(sb0 + k0 + e) : 0.f;
-          const float b1 = in && two ? __ldg(sb0 + p.k_blocks + k0 + e) : 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            dst[(2 * e) * 128 + 32 * i] = a[i][e] * b0;
-            dst[(2 * e + 1) * 128 + 32 * i] = a[i][e] * b1;
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&C.scale_full[buf]));
-        if (++buf == 2) {
-          buf = 0;
-          ++round;
-        }
-      }
-    }
-  }
   } else {
     setmaxnreg_inc<kEpiRegs>();
     // ------------------------------------------------------------ epilogue (both CTAs)
@@ -359,52 +366,55 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     constexpr int kOutCols = 64 / (int)sizeof(T);  // columns of a staged 64-byte row
     constexpr int kVec = 16 / (int)sizeof(T);
     const float* my_scale = sScale + half * 128 + quad * 32 + lane;
-    int buf = 0, chunk = 0;  // accumulator and scale chunk in use
-    uint32_t round = 0, chunk_round = 0;
+    const uint32_t cols0 = tmem + lane_base + half * kPairAccCols;  // + 2 * kPairAccCols for buffer 1
+    const uint32_t acc_full = smem_u32(&C.acc_full[half]);          // + 16 bytes for buffer 1
+    const uint32_t scale_full = smem_u32(&C.scale_full[0]);
+    int chunk = 0;  // scale chunk in use
+    uint32_t it = 0, chunk_round = 0;
     bool ok = true;
     for (int64_t t = pair; ok && t < total_tiles; t += pairs) {
-      float acc[128];
+      uint64_t acc[64];
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-      for (int kb = 0; kb < p.k_blocks; ++kb) {
-        bool got = true;
-        if (kb % kChunk == 0)
-          got = mbar_wait(smem_u32(&C.scale_full[chunk]), chunk_round & 1u, abort_flag, p.status, 436);
-        const float scale = my_scale[chunk * kChunkFloats + (kb % kChunk) * 256];
-        got = got && mbar_wait(smem_u32(&C.acc_full[2 * buf + half]), round & 1u, abort_flag, p.status, 434);
-        if (!__all_sync(0xffffffffu, got)) {
+      for (int i = 0; i < 64; ++i) acc[i] = 0;
+      for (int left = p.k_blocks; left > 0; left -= kChunk) {
+        if (!wait_warp(scale_full + chunk * 8, chunk_round & 1u, abort_flag, p.status, 436)) {
           ok = false;
           break;
         }
-        tc_fence_after();
-        const uint32_t col0 = tmem + lane_base + (2 * buf + half) * kPairAccCols;
-        // The load of the next 32 columns is in flight while 32 are added.
-        uint32_t r[2][32];
-        tmem_ld32(col0, r[0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_wait_ld();
-          if (c < 3) {
-            tmem_ld32(col0 + 32 * (c + 1), r[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 16);
+        const float* chunk_scale = my_scale + chunk * kChunkFloats;
+        const int in_chunk = min(left, kChunk);
+#pragma unroll 2
+        for (int e = 0; e < in_chunk; ++e, ++it) {
+          const uint32_t buf = it & 1u;  // accumulator
+          const float scale = chunk_scale[e * 256];
+          if (!wait_warp(acc_full + buf * 16, (it >> 1) & 1u, abort_flag, p.status, 434)) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
+          const uint32_t col0 = cols0 + buf * 2 * kPairAccCols;
+          const uint64_t s2 = f2_pack(scale, scale);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(r[c & 1][i]), scale, acc[32 * c + i]);
-        }
-        if (++buf == 2) {
-          buf = 0;
-          ++round;
-        }
-        if (kb % kChunk == kChunk - 1 || kb == p.k_blocks - 1) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&C.scale_empty[chunk]));
-          if (++chunk == 2) {
-            chunk = 0;
-            ++chunk_round;
+          for (int c = 0; c < 8; ++c) {
+            uint32_t r[16];
+            tmem_ld16(col0 + 16 * c, r);
+            tmem_wait_ld();
+            if (c == 7) {  // all of this half is in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              acc[8 * c + i] = f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s2, acc[8 * c + i]);
           }
+        }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&C.scale_empty[chunk]));
+        if (++chunk == 2) {
+          chunk = 0;
+          ++chunk_round;
         }
       }
       if (!ok) break;
@@ -426,7 +436,7 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
         for (int q = 0; q < 4; ++q) {  // 16 bytes of the row at a time
           float f[kVec];
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) f[i] = acc[g * kOutCols + q * kVec + i];
+          for (int i = 0; i < kVec / 2; ++i) f2_unpack(acc[(g * kOutCols + q * kVec) / 2 + i], f[2 * i], f[2 * i + 1]);
           finish_columns<T>(p, m, row_ok, nc + q * kVec, f);
           if (p.tma_out) {
             uint32_t w[4];
@@ -475,7 +485,7 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
 }
 
 // ------------------------------------------------------------------ few rows: plain streaming
-// For up to four rows of A the product is the reading of B once: each thread multiplies its 16
+// For one or two rows of A the product is the reading of B once: each thread multiplies its 16
 // bytes of a weight row with its 16 columns of the M rows, which it keeps as fp32, so weights go
 // from global memory to registers with no staging, and no TMEM, barrier or tensor map has to be
 // set up.  A CTA of 8 warps takes kRows weight rows per row group; `kWarps` warps split K (512
@@ -501,7 +511,6 @@ __global__ void __launch_bounds__(kStreamThreads) fp8_gemm_blocks_stream_kernel(
                                                                                 int k_warps, BlockGemmParams p) {
   __shared__ float part[kStreamThreads / 32][kRows * M];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rows = (int)p.M;  // at most M
   const int group = warp / k_warps, kw = warp - group * k_warps;
   const int n0 = (blockIdx.x * (kStreamThreads / 32 / k_warps) + group) * kRows;
   float acc[kRows * M];  // [row][m]
@@ -518,11 +527,11 @@ __global__ void __launch_bounds__(kStreamThreads) fp8_gemm_blocks_stream_kernel(
       const float s = __ldg(sb + kb);
       float sm[M];
 #pragma unroll
-      for (int m = 0; m < M; ++m) sm[m] = s * __ldg(p.a_scale + min(m, rows - 1) * p.a_row_stride + kb * p.a_block_stride);
+      for (int m = 0; m < M; ++m) sm[m] = s * __ldg(p.a_scale + m * p.a_row_stride + kb * p.a_block_stride);
       float x[M][16];
 #pragma unroll
       for (int m = 0; m < M; ++m)
-        e4m3x16_to_float(__ldg(reinterpret_cast<const uint4*>(a + (int64_t)min(m, rows - 1) * p.K + k)), x[m]);
+        e4m3x16_to_float(__ldg(reinterpret_cast<const uint4*>(a + (int64_t)m * p.K + k)), x[m]);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         float y[16];
@@ -558,14 +567,14 @@ __global__ void __launch_bounds__(kStreamThreads) fp8_gemm_blocks_stream_kernel(
       acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
     }
   }
-  // kRows * M is 8, 16 or 32: one value per lane, held by 4, 2 or 1 lanes
+  // kRows * M is 8 or 16: one value per lane, held by 4 or 2 lanes
   if (lane % (32 / (kRows * M)) == 0) part[warp][index] = acc[0];
   __syncthreads();
   const int groups = kStreamThreads / 32 / k_warps;
   for (int i = threadIdx.x; i < groups * kRows * M; i += kStreamThreads) {
     const int g = i / (kRows * M), e = i - g * (kRows * M);
     const int n = (blockIdx.x * groups + g) * kRows + e / M, m = e % M;
-    if (n >= p.N || m >= rows) continue;
+    if (n >= p.N) continue;
     float f = 0.f;
     for (int w = 0; w < k_warps; ++w) f += part[g * k_warps + w][e];
     if (p.bias != nullptr) f += __ldg(p.bias + n);
@@ -576,17 +585,33 @@ __global__ void __launch_bounds__(kStreamThreads) fp8_gemm_blocks_stream_kernel(
   }
 }
 
+int sm_count() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
 template <typename T>
 int launch_stream(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, cudaStream_t s) {
+  // Warps along K: the fewest passes over K times waves of CTAs (about four CTAs per SM).
   int k_warps = 1;
-  while (k_warps < 8 && k_warps * 512 < p.K) k_warps *= 2;
+  int64_t best = 0;
+  for (int w = 1; w <= 8; w *= 2) {
+    const int64_t passes = (p.K + 512 * w - 1) / (512 * w);
+    const int64_t ctas = (p.N + kRows * (8 / w) - 1) / (kRows * (8 / w));
+    const int64_t cost = passes * ((ctas + 4 * sm_count() - 1) / (4 * sm_count()));
+    if (w == 1 || cost < best) {
+      best = cost;
+      k_warps = w;
+    }
+  }
   const int rows = kRows * (kStreamThreads / 32 / k_warps);
   const unsigned grid = (unsigned)((p.N + rows - 1) / rows);
-  switch (p.M) {
-    case 1: fp8_gemm_blocks_stream_kernel<T, 1><<<grid, kStreamThreads, 0, s>>>(a, b, k_warps, p); break;
-    case 2: fp8_gemm_blocks_stream_kernel<T, 2><<<grid, kStreamThreads, 0, s>>>(a, b, k_warps, p); break;
-    default: fp8_gemm_blocks_stream_kernel<T, 4><<<grid, kStreamThreads, 0, s>>>(a, b, k_warps, p); break;
-  }
+  if (p.M == 1)
+    fp8_gemm_blocks_stream_kernel<T, 1><<<grid, kStreamThreads, 0, s>>>(a, b, k_warps, p);
+  else
+    fp8_gemm_blocks_stream_kernel<T, 2><<<grid, kStreamThreads, 0, s>>>(a, b, k_warps, p);
   SB_CHECK_LAUNCH("sb_fp8_gemm_blocks launch");
   return SB_OK;
 }
@@ -632,20 +657,20 @@ int make_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* b
 }
 
 // ------------------------------------------------------------------ some rows: weights as MMA rows
-// A tile is 128 weight rows (the MMA's M) x T rows of A (its N, a multiple of 16 up to 128), so a
+// A tile is 128 weight rows (the MMA's M) x T rows of A (its N, a multiple of 16 up to 64), so a
 // few rows of A do not fill a 256-row tile with padding.  CTAs are small and several share an SM,
 // which hides each one's set-up and hand-overs behind the others' loads; where the tiles alone do
 // not fill the GPU, the CTAs of a cluster split K and add their sums, in rank order, through
 // distributed shared memory.  Thread = weight row: the scale of accumulator column j is
 // a_scale[row j] * b_scale, read from shared memory by all lanes at once.
-//   warps 0 .. EW-1 epilogue (EW 4: all columns; EW 8: warps 4-7 take the upper half), then the
-//   TMA producer, the MMA issuer and the scale warp.
+constexpr int kSwapProducer = 4, kSwapIssuer = 5, kSwapScales = 6;  // warps 0-3: epilogue
+constexpr int kSwapThreads = 224;
+constexpr int kSwapTokens = 64;
 constexpr int kSwapMaxStages = 4;
-constexpr int kSwapRing = 4;  // TMEM buffers at most
 
 struct __align__(8) SwapControl {
   uint64_t full[kSwapMaxStages], empty[kSwapMaxStages];
-  uint64_t acc_full[kSwapRing], acc_empty[kSwapRing];
+  uint64_t acc_full[2], acc_empty[2];
   uint64_t scale_full[2], scale_empty[2];
   uint64_t mma_done;
   uint32_t tmem_base;
@@ -656,8 +681,9 @@ struct SwapShape {
   int tokens;      // T: rows of A per tile
   int m_tiles;
   int splits;      // CTAs of a cluster
-  int stages, ring;
-  uint32_t acc_stride;  // TMEM columns per buffer; ring * acc_stride are allocated
+  int group;       // k-blocks per stage and per TMEM buffer
+  int stages;
+  uint32_t acc_stride;  // TMEM columns per k-block; 2 * group * acc_stride are allocated
 };
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
@@ -687,14 +713,15 @@ __device__ __forceinline__ void finish_value(const BlockGemmParams& p, int64_t m
   static_cast<T*>(p.out)[at] = Elem<T>::from_f(f);
 }
 
-template <typename T, int EW, int CW>
-__global__ void __launch_bounds__(32 * (EW + 3), 2)
+template <typename T, int CW>
+__global__ void __launch_bounds__(kSwapThreads, 2)
 fp8_gemm_blocks_swap_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                             BlockGemmParams p, SwapShape q) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const bool aligned = (smem_u32(smem) & 1023u) == 0u;  // alike in every CTA
   const int tokens = q.tokens;
-  const int stage_bytes = kPairOpBytes + tokens * kBlockK;
+  const int span_bytes = kPairOpBytes + tokens * kBlockK;  // a k-block's weights and rows of A
+  const int stage_bytes = q.group * span_bytes;
   float* sScale = reinterpret_cast<float*>(smem + q.stages * stage_bytes);  // [2][kChunk][tokens]
   SwapControl& C = *reinterpret_cast<SwapControl*>(sScale + 2 * kChunk * tokens);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -712,20 +739,18 @@ fp8_gemm_blocks_swap_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       mbar_init(smem_u32(&C.full[s]), 1);
       mbar_init(smem_u32(&C.empty[s]), 1);
     }
-    for (int b = 0; b < kSwapRing; ++b) {
-      mbar_init(smem_u32(&C.acc_full[b]), 1);
-      mbar_init(smem_u32(&C.acc_empty[b]), EW);
-    }
     for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&C.acc_full[b]), 1);
+      mbar_init(smem_u32(&C.acc_empty[b]), 4);
       mbar_init(smem_u32(&C.scale_full[b]), 1);
-      mbar_init(smem_u32(&C.scale_empty[b]), EW);
+      mbar_init(smem_u32(&C.scale_empty[b]), 4);
     }
     mbar_init(smem_u32(&C.mma_done), 1);
     C.abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == EW + 1) {
-    tmem_alloc(smem_u32(&C.tmem_base), q.ring * q.acc_stride);
+  if (warp == kSwapIssuer) {
+    tmem_alloc(smem_u32(&C.tmem_base), 2 * q.group * q.acc_stride);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -739,21 +764,23 @@ fp8_gemm_blocks_swap_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
 #pragma unroll
   for (int i = 0; i < CW; ++i) acc[i] = 0.f;
   const int quad = warp & 3;
-  const int col0 = EW == 8 && warp >= 4 ? (tokens + 31) / 32 * 16 : 0;
-  const int cols = EW == 8 ? (warp >= 4 ? tokens - col0 : (tokens + 31) / 32 * 16) : tokens;
 
-  if (warp == EW) {
+  if (warp == kSwapProducer) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
       int s = 0;
       uint32_t use = 0;
       int issued = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0; kb < kb1; kb += q.group) {
         if (!mbar_wait(smem_u32(&C.empty[s]), (use & 1u) ^ 1u, abort_flag, p.status, 441)) break;
-        const uint32_t st = base + s * stage_bytes, full = smem_u32(&C.full[s]);
-        mbar_arrive_expect_tx(full, stage_bytes);
-        tma_load_2d(st, &tm_b, full, kb * kBlockK, nt * 128);
-        tma_load_2d(st + kPairOpBytes, &tm_a, full, kb * kBlockK, mt * tokens);
+        const uint32_t full = smem_u32(&C.full[s]);
+        const int g = min(q.group, kb1 - kb);
+        mbar_arrive_expect_tx(full, g * span_bytes);
+        for (int i = 0; i < g; ++i) {  // g * 128 consecutive bytes of each weight row
+          const uint32_t st = base + s * stage_bytes + i * span_bytes;
+          tma_load_2d(st, &tm_b, full, (kb + i) * kBlockK, nt * 128);
+          tma_load_2d(st + kPairOpBytes, &tm_a, full, (kb + i) * kBlockK, mt * tokens);
+        }
         ++issued;
         if (++s == q.stages) {
           s = 0;
@@ -763,37 +790,41 @@ fp8_gemm_blocks_swap_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       for (int st = 0; st < q.stages; ++st)
         if (issued > st) mbar_drain(smem_u32(&C.full[st]), (uint32_t)(((issued - 1 - st) / q.stages) & 1));
     }
-  } else if (warp == EW + 1) {
+  } else if (warp == kSwapIssuer) {
     // ------------------------------------------------------------ MMA issuer
     if (elect_one()) {
       const uint32_t idesc = idesc_e4m3_f32(128, tokens);
       const uint64_t desc0 = smem_desc_sw128(base, 16, 1024);
       int s = 0, buf = 0;
       uint32_t use = 0, round = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0; kb < kb1; kb += q.group) {
         if (!mbar_wait(smem_u32(&C.full[s]), use & 1u, abort_flag, p.status, 442) ||
             !mbar_wait(smem_u32(&C.acc_empty[buf]), (round & 1u) ^ 1u, abort_flag, p.status, 443))
           break;
         tc_fence_after();
-        const uint64_t dw = desc0 + (uint64_t)((s * stage_bytes) >> 4);
-        const uint64_t dx = dw + (uint64_t)(kPairOpBytes >> 4);
+        const int g = min(q.group, kb1 - kb);
+        for (int i = 0; i < g; ++i) {
+          const uint64_t dw = desc0 + (uint64_t)((s * stage_bytes + i * span_bytes) >> 4);
+          const uint64_t dx = dw + (uint64_t)(kPairOpBytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kBlockK / 32; ++kk)
-          mma_f8(tmem + buf * q.acc_stride, dw + (uint64_t)(kk * 2), dx + (uint64_t)(kk * 2), idesc, kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < kBlockK / 32; ++kk)
+            mma_f8(tmem + (buf * q.group + i) * q.acc_stride, dw + (uint64_t)(kk * 2), dx + (uint64_t)(kk * 2), idesc,
+                   kk > 0 ? 1u : 0u);
+        }
         tc_commit(smem_u32(&C.acc_full[buf]));
         tc_commit(smem_u32(&C.empty[s]));
         if (++s == q.stages) {
           s = 0;
           ++use;
         }
-        if (++buf == q.ring) {
+        if (++buf == 2) {
           buf = 0;
           ++round;
         }
       }
       tc_commit(smem_u32(&C.mma_done));
     }
-  } else if (warp == EW + 2) {
+  } else if (warp == kSwapScales) {
     // ------------------------------------------------------------ scales
     const float* sb = p.b_scale + (int64_t)nt * p.k_blocks;
     int buf = 0;
@@ -821,78 +852,76 @@ fp8_gemm_blocks_swap_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   } else {
     // ------------------------------------------------------------ epilogue
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    int buf = 0, chunk = 0;
-    uint32_t round = 0, chunk_round = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const int e = (kb - kb0) % kChunk;
-      bool got = true;
-      if (e == 0) got = mbar_wait(smem_u32(&C.scale_full[chunk]), chunk_round & 1u, abort_flag, p.status, 445);
-      got = got && mbar_wait(smem_u32(&C.acc_full[buf]), round & 1u, abort_flag, p.status, 446);
-      if (!__all_sync(0xffffffffu, got)) break;
-      tc_fence_after();
-      const float4* scale = reinterpret_cast<const float4*>(sScale + (chunk * kChunk + e) * tokens + col0);
-      const uint32_t src = tmem + lane_base + buf * q.acc_stride + col0;
+    const uint32_t acc_full = smem_u32(&C.acc_full[0]), scale_full = smem_u32(&C.scale_full[0]);
+    uint32_t it = 0;  // groups done: buffer it & 1
+    for (int k0 = kb0; k0 < kb1; k0 += kChunk) {
+      const uint32_t chunks = (uint32_t)(k0 - kb0) / kChunk, chunk = chunks & 1u;
+      if (!wait_warp(scale_full + chunk * 8, (chunks >> 1) & 1u, abort_flag, p.status, 445)) break;
+      const int in_chunk = min(kb1 - k0, kChunk);
+      bool ok = true;
+      for (int e0 = 0; e0 < in_chunk; e0 += q.group, ++it) {  // groups divide chunks
+        const uint32_t buf = it & 1u;
+        ok = wait_warp(acc_full + buf * 8, (it >> 1) & 1u, abort_flag, p.status, 446);
+        if (!ok) break;
+        tc_fence_after();
+        const int g = min(q.group, in_chunk - e0);
+        const float4* scale = reinterpret_cast<const float4*>(sScale + (chunk * kChunk + e0) * tokens);
+        uint32_t src = tmem + lane_base + buf * q.group * q.acc_stride;
+        for (int k = 0; k < g; ++k, scale += tokens / 4, src += q.acc_stride) {
 #pragma unroll
-      for (int c = 0; c < CW; c += 16) {
-        if (c < cols) {
-          uint32_t r[16];
-          tmem_ld16(src + c, r);
-          tmem_wait_ld();
+          for (int c = 0; c < CW; c += 16) {
+            if (c < tokens) {
+              uint32_t r[16];
+              tmem_ld16(src + c, r);
+              tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 s = scale[c / 4 + i];
-            acc[c + 4 * i + 0] = fmaf(__uint_as_float(r[4 * i + 0]), s.x, acc[c + 4 * i + 0]);
-            acc[c + 4 * i + 1] = fmaf(__uint_as_float(r[4 * i + 1]), s.y, acc[c + 4 * i + 1]);
-            acc[c + 4 * i + 2] = fmaf(__uint_as_float(r[4 * i + 2]), s.z, acc[c + 4 * i + 2]);
-            acc[c + 4 * i + 3] = fmaf(__uint_as_float(r[4 * i + 3]), s.w, acc[c + 4 * i + 3]);
+              for (int i = 0; i < 4; ++i) {
+                const float4 s = scale[c / 4 + i];
+                acc[c + 4 * i + 0] = fmaf(__uint_as_float(r[4 * i + 0]), s.x, acc[c + 4 * i + 0]);
+                acc[c + 4 * i + 1] = fmaf(__uint_as_float(r[4 * i + 1]), s.y, acc[c + 4 * i + 1]);
+                acc[c + 4 * i + 2] = fmaf(__uint_as_float(r[4 * i + 2]), s.z, acc[c + 4 * i + 2]);
+                acc[c + 4 * i + 3] = fmaf(__uint_as_float(r[4 * i + 3]), s.w, acc[c + 4 * i + 3]);
+              }
+            }
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&C.acc_empty[buf]));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&C.acc_empty[buf]));
-      if (++buf == q.ring) {
-        buf = 0;
-        ++round;
-      }
-      if (e == kChunk - 1 || kb == kb1 - 1) {
-        if (lane == 0) mbar_arrive(smem_u32(&C.scale_empty[chunk]));
-        if (++chunk == 2) {
-          chunk = 0;
-          ++chunk_round;
-        }
-      }
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(smem_u32(&C.scale_empty[chunk]));
     }
     const int n = nt * 128 + quad * 32 + lane;
     if (q.splits == 1) {
       if (n < p.N) {
 #pragma unroll
         for (int j = 0; j < CW; ++j) {
-          const int64_t m = (int64_t)mt * tokens + col0 + j;
-          if (j < cols && m < p.M) finish_value<T>(p, m, n, acc[j]);
+          const int64_t m = (int64_t)mt * tokens + j;
+          if (j < tokens && m < p.M) finish_value<T>(p, m, n, acc[j]);
         }
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == EW + 1) {
+  if (warp == kSwapIssuer) {
     tc_fence_after();
     mbar_drain(smem_u32(&C.mma_done), 0);
-    tmem_dealloc(tmem, q.ring * q.acc_stride);
+    tmem_dealloc(tmem, 2 * q.group * q.acc_stride);
   }
   if (q.splits > 1) {
     // Every stage has been read: the stages hold this CTA's sums as [column][weight row].
     __syncthreads();
     float* part = reinterpret_cast<float*>(smem);
-    if (warp < EW) {
+    if (warp < 4) {
 #pragma unroll
       for (int j = 0; j < CW; ++j)
-        if (j < cols) part[(col0 + j) * 128 + quad * 32 + lane] = acc[j];
+        if (j < tokens) part[j * 128 + quad * 32 + lane] = acc[j];
     }
     cluster_sync_all();
     const int per = tokens / q.splits;  // columns this CTA finishes; splits divides 16
-    for (int i = threadIdx.x; i < per * 128; i += 32 * (EW + 3)) {
+    for (int i = threadIdx.x; i < per * 128; i += kSwapThreads) {
       const int j = rank * per + i / 128, row = i % 128;
       float f = 0.f;
       for (int r = 0; r < q.splits; ++r)
@@ -905,12 +934,6 @@ fp8_gemm_blocks_swap_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
 
 template <typename T>
 int launch_pair(const uint8_t* a, const uint8_t* b, BlockGemmParams p, cudaStream_t s) {
@@ -948,20 +971,20 @@ int launch_pair(const uint8_t* a, const uint8_t* b, BlockGemmParams p, cudaStrea
   return SB_OK;
 }
 
-template <typename T, int EW, int CW>
+template <typename T, int CW>
 int launch_swap(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, SwapShape q, cudaStream_t s) {
   CUtensorMap ma, mb;
   int rc;
   if ((rc = make_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a, p.K, p.M, q.tokens, true)) != SB_OK) return rc;
   if ((rc = make_map(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b, p.K, p.N, 128, true)) != SB_OK) return rc;
-  const size_t smem = (size_t)q.stages * (kPairOpBytes + q.tokens * kBlockK) + (size_t)2 * kChunk * q.tokens * 4 +
+  const size_t smem = (size_t)q.stages * q.group * (kPairOpBytes + q.tokens * kBlockK) + (size_t)2 * kChunk * q.tokens * 4 +
                       sizeof(SwapControl);
-  auto kernel = fp8_gemm_blocks_swap_kernel<T, EW, CW>;
+  auto kernel = fp8_gemm_blocks_swap_kernel<T, CW>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (err != cudaSuccess) return cuda_error(err, "sb_fp8_gemm_blocks: set smem");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)q.m_tiles * ((p.N + 127) / 128) * q.splits), 1, 1);
-  cfg.blockDim = dim3(32 * (EW + 3), 1, 1);
+  cfg.blockDim = dim3(kSwapThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -977,22 +1000,76 @@ int launch_swap(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, Sw
   return SB_OK;
 }
 
-template <typename T>
-int dispatch_swap(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, cudaStream_t s) {
+// Which kernel, and its shape.  The estimates are fits (in us, within about 20 %) of times measured
+// on one B200 with K of 4096 to 16384 and weights that come from HBM:
+//   pair: 6 + 0.45 per k-block and wave of tiles (one 256 x 256 tile per CTA pair);
+//   swap: 6 + 0.55 (up to 32 rows: 0.30) per k-block of a CTA with one CTA per SM, 0.70 (0.55) with
+//         two, + 3 where a cluster adds up its splits.
+// Both sides at M x N x K: 64 x 4096 x 4096 swap 11.5, pair 20.1; 1000 x 392 x 4112 15.0, 22.5;
+// 64 x 28672 x 5376 36.5, 47; 256 x 4096 x 4096 22.5, 20.1; 128 x 14336 x 5376 34.9, 29.6.
+double pair_estimate(int64_t M, int N, int k_blocks, int sms) {
+  const int64_t tiles = (M + 255) / 256 * ((N + 255) / 256), pairs = sms / 2;
+  return 6.0 + 0.45 * (double)((tiles + pairs - 1) / pairs) * k_blocks;
+}
+
+double swap_shape(int64_t M, int N, int k_blocks, int sms, SwapShape* shape) {
   SwapShape q{};
-  q.m_tiles = (int)((p.M + 127) / 128);
-  q.tokens = (int)((p.M + q.m_tiles - 1) / q.m_tiles + 15) / 16 * 16;
-  const int64_t tiles = (int64_t)q.m_tiles * ((p.N + 127) / 128);
-  // Split K until there are two CTAs per SM, each with at least four k-blocks.
-  q.splits = 1;
-  while (q.splits < 8 && tiles * q.splits < 2 * sm_count() && p.k_blocks >= 8 * q.splits) q.splits *= 2;
-  q.stages = q.tokens <= 16 ? 4 : 3;
-  q.acc_stride = q.tokens <= 32 ? 32 : q.tokens <= 64 ? 64 : 128;
-  q.ring = q.tokens <= 32 ? 4 : 2;
-  if (q.tokens <= 16) return launch_swap<T, 4, 16>(a, b, p, q, s);
-  if (q.tokens <= 32) return launch_swap<T, 4, 32>(a, b, p, q, s);
-  if (q.tokens <= 64) return launch_swap<T, 4, 64>(a, b, p, q, s);
-  return launch_swap<T, 8, 64>(a, b, p, q, s);
+  q.m_tiles = (int)((M + kSwapTokens - 1) / kSwapTokens);
+  q.tokens = (int)(((M + q.m_tiles - 1) / q.m_tiles + 15) / 16 * 16);
+  const bool narrow = q.tokens <= 32;
+  const int64_t tiles = (int64_t)q.m_tiles * ((N + 127) / 128);
+  double best = 0;
+  // Splits of K by 1, 2, 4 or 8, each of at least eight k-blocks; two CTAs per SM are resident.
+  for (int splits = 1; splits <= 8 && (splits == 1 || k_blocks >= 8 * splits); splits *= 2) {
+    const int64_t ctas = tiles * splits;
+    const int64_t waves = (ctas + 2 * sms - 1) / (2 * sms);
+    const bool one = ctas <= sms;
+    const double t = 6.0 + (splits > 1 ? 3.0 : 0.0) +
+                     (one ? (narrow ? 0.30 : 0.55) : (narrow ? 0.55 : 0.70)) * (double)waves * k_blocks / splits;
+    if (splits == 1 || t < best) {
+      best = t;
+      q.splits = splits;
+      // Two k-blocks per stage read 256 consecutive bytes of each weight row and halve the
+      // hand-overs; with two CTAs per SM the stages of a CTA have to fit 113 KB.
+      q.group = one || narrow ? 2 : 1;
+      q.stages = one ? (narrow ? 4 : 3) : (narrow ? 2 : 4);
+    }
+  }
+  q.acc_stride = narrow ? 32 : 64;
+  *shape = q;
+  return best;
+}
+
+template <typename T>
+int dispatch(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, cudaStream_t s) {
+  // One or two rows: streaming starts sooner, swap reads faster (256-byte bursts by TMA).  Measured
+  // at one row (stream, swap): 1024 x 1024 3.3, 5.8; 4096 x 4096 5.9, 7.3; 4096 x 16384 18.3, 16.6;
+  // 14336 x 5376 24.5, 16.9; 28672 x 5376 42.4, 28.5.
+  if (p.M <= 2 && (int64_t)p.N * p.K <= (24 << 20)) return launch_stream<T>(a, b, p, s);
+  const int sms = sm_count();
+  SwapShape q{};
+  const double pair = pair_estimate(p.M, p.N, p.k_blocks, sms);
+  // An estimate of swap beyond 2048 rows would never win, and its grid would outgrow 32 bits.
+  if (p.M <= 2048 && swap_shape(p.M, p.N, p.k_blocks, sms, &q) < pair) {
+    if (q.tokens <= 16) return launch_swap<T, 16>(a, b, p, q, s);
+    if (q.tokens <= 32) return launch_swap<T, 32>(a, b, p, q, s);
+    return launch_swap<T, 64>(a, b, p, q, s);
+  }
+  // A few rows past whole 256-row tiles can cost a wave of nearly empty tiles: they get a launch
+  // of their own where that is cheaper (259 x 28672 x 5376: 99 us as one launch).
+  const int64_t rest = p.M % 256, whole = p.M - rest;
+  if (whole > 0 && rest > 0 && rest <= kSwapTokens &&
+      pair_estimate(whole, p.N, p.k_blocks, sms) + swap_shape(rest, p.N, p.k_blocks, sms, &q) < pair) {
+    BlockGemmParams head = p, tail = p;
+    head.M = whole;
+    tail.M = rest;
+    tail.a_scale += whole * p.a_row_stride;
+    tail.out = static_cast<T*>(p.out) + whole * p.N;
+    if (p.residual != nullptr) tail.residual = static_cast<const T*>(p.residual) + whole * p.N;
+    const int rc = launch_pair<T>(a, b, head, s);
+    return rc != SB_OK ? rc : dispatch<T>(a + whole * p.K, b, tail, s);
+  }
+  return launch_pair<T>(a, b, p, s);
 }
 
 }  // namespace
@@ -1034,9 +1111,5 @@ extern "C" int sb_fp8_gemm_blocks(const uint8_t* a, const float* a_scale, int64_
   p.a_vec = a_block_stride == 1 && a_row_stride % 4 == 0 && (uintptr_t)a_scale % 16 == 0;
   p.tma_out = (int64_t)N * (out_dtype == SB_BF16 ? 2 : 4) % 16 == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  if (M <= 4)
-    return out_dtype == SB_BF16 ? launch_stream<__nv_bfloat16>(a, b, p, s) : launch_stream<float>(a, b, p, s);
-  if (M <= 1024)
-    return out_dtype == SB_BF16 ? dispatch_swap<__nv_bfloat16>(a, b, p, s) : dispatch_swap<float>(a, b, p, s);
-  return out_dtype == SB_BF16 ? launch_pair<__nv_bfloat16>(a, b, p, s) : launch_pair<float>(a, b, p, s);
+  return out_dtype == SB_BF16 ? dispatch<__nv_bfloat16>(a, b, p, s) : dispatch<float>(a, b, p, s);
 }

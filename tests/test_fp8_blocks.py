@@ -367,7 +367,8 @@ def assert_gemm(out, want, error):
 
 GEMM_SIZES = [(1, 1, 16), (1, 4096, 4096), (2, 130, 144), (2, 4104, 5376), (3, 1000, 512), (3, 77, 10000), (4, 392, 4112), (4, 5, 16), (8, 512, 128), (9, 1420, 2000), (17, 392, 4112), (24, 1000, 5376),
               (33, 129, 256), (64, 2056, 1024), (65, 640, 640), (100, 4096, 400), (128, 257, 16384), (129, 128, 272),
-              (200, 3000, 1040), (256, 256, 128), (259, 5376, 1360), (513, 264, 2064), (1000, 392, 4112), (2100, 4104, 912)]
+              (200, 3000, 1040), (256, 256, 128), (259, 5376, 1360), (513, 264, 2064), (1000, 392, 4112), (2100, 4104, 912),
+              (1, 28672, 1040), (2, 8200, 4096), (259, 28672, 5376), (2110, 5000, 1040)]
 
 
 @pytest.mark.gpu
