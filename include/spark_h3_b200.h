@@ -387,13 +387,14 @@ int sb_fp8_quantize_segments(const void* x, int64_t M, int K, int seg, int64_t s
 /*
  * e4m3 quantisers with one scale per row and 128 columns (no counterpart in the reference, whose
  * scales are per token or per tensor): for columns [128 b, 128 b + 128) of row m (the last block
- * may be short), scales[m, b] = max(absmax * fp32(1/448), 1e-12) and out = e4m3(y * (1 / scale)),
+ * may be short), scales[m, b] = max(absmax * fp32(1/448), 1e-12) and out = e4m3(y / scale),
  * y being x, a * g * sigmoid(g) of a [M, 2K] projection output (value half first), or GELU(x)
- * (erf form), evaluated in fp32.  A code equals e4m3(y / scale) except where that quotient lies
- * within 2^-23 of itself from the middle of two codes.  A NaN makes its whole block NaN; an
+ * (erf form), evaluated in fp32.  The quotient is formed with a reciprocal and is off by less
+ * than 2^-22 of itself: a code can be the neighbour of the nearest one where the quotient lies
+ * that close to the middle of the two.  A NaN makes its whole block NaN; an
  * infinity makes its block's finite values 0.
- * x: rows of K (swiglu: 2K) columns, x_stride elements apart (dtype); any alignment of its
- * elements, 16-byte loads where every row starts on a 16-byte boundary and K % 8 == 0.
+ * x: rows of K (swiglu: 2K) columns, x_stride elements apart (dtype), aligned to its elements;
+ * vector loads where K, the stride and the pointers are multiples of four elements.  K <= 2^24.
  * out: [M, K] bytes; scales: [M, ceil(K / 128)] fp32.
  */
 int sb_fp8_quantize_blocks(const void* x, int64_t x_stride, int dtype, int64_t M, int K, uint8_t* out,
@@ -408,7 +409,7 @@ int sb_fp8_gelu_quantize_blocks(const void* x, int64_t x_stride, int dtype, int6
  * the reference):
  *   s = residual + gate * x            (fp32; stored rounded to the dtype as `summed`)
  *   y = s * rsqrt(mean(s^2) + eps) * weight + shift
- *   out = e4m3(y * (1 / scale)),  scale = max(absmax(y) * fp32(1/448), 1e-12)
+ *   out = e4m3(y / scale) (as above),  scale = max(absmax(y) * fp32(1/448), 1e-12)
  * with one scale per row (blocks 0, scales [M]: the operand of sb_fp8_gemm) or per row and 128
  * columns (blocks 1, scales [M, ceil(C / 128)]: the operand of sb_fp8_gemm_blocks).  The norm
  * works on the unrounded sum.  residual and summed are both NULL (s = x) or both given; summed

@@ -2,7 +2,8 @@
 against their definition in 64 bits.
 
 Tolerances.  A code is the nearest e4m3 value of y / scale, where the kernel's quotient may be off
-by `slack` of itself: 2^-23 from the reciprocal and the product, plus the error of the fp32 y.
+by `slack` of itself: 2^-22 from the reciprocal (2^-23) and the product (2^-24), plus the error of the
+fp32 y.
 A GEMM sums blocks of 128 exact products in fp32: each of the 128 + blocks additions rounds (or
 truncates) to at most 2^-23 of the sum of the terms' magnitudes; its output then rounds once
 (eps / 2 of the value)."""
@@ -92,7 +93,7 @@ def test_quantisers_reject_bad_arguments(entry, halves):
     lib = _lib.load()
     valid = dict(x=_P, stride=256 * halves, dtype=1, M=4, K=256, out=_P, scales=_P, stream=None)
     for change, message in ((dict(x=None), "null pointer"), (dict(scales=None), "null pointer"),
-                            (dict(dtype=2), "bad dtype"), (dict(M=0), "M in [1, 2^31)"), (dict(K=0), "K in [1, 2^30]"),
+                            (dict(dtype=2), "bad dtype"), (dict(M=0), "M in [1, 2^31)"), (dict(K=0), "K in [1, 2^24]"),
                             (dict(stride=256 * halves - 1), "rows overlap"), (dict(x=_P + 1), "aligned to their elements"),
                             (dict(scales=_P + 2), "aligned to their elements")):
         assert getattr(lib, entry)(*{**valid, **change}.values()) == -1, change
@@ -167,7 +168,7 @@ def check_quantised(codes, scale, y, y_error):
     assert bool(((scale.double() - want).abs() <= want * 2.0 ** -23 + group_absmax(y_error) / 448).all())
     s = spread(scale.double(), K)
     q = y / s
-    assert_nearest_codes(codes, q, 2.0 ** -23 + (y_error / s) / q.abs().clamp_min(1e-30))
+    assert_nearest_codes(codes, q, 2.0 ** -22 + (y_error / s) / q.abs().clamp_min(1e-30))
 
 
 @pytest.mark.gpu
@@ -281,7 +282,7 @@ def test_add_rms_norm_quantize(cuda_device, dtype, blocks, M, C, residual, gate,
         want = (y.abs().amax(dim=1, keepdim=True) / 448).clamp_min(1e-12)
         assert bool(((scale.double() - want).abs() <= want * 2.0 ** -23 + error.amax(dim=1, keepdim=True) / 448).all())
         q = y / scale.double()
-        assert_nearest_codes(codes, q, 2.0 ** -23 + (error / scale.double()) / q.abs().clamp_min(1e-30))
+        assert_nearest_codes(codes, q, 2.0 ** -22 + (error / scale.double()) / q.abs().clamp_min(1e-30))
 
 
 @pytest.mark.gpu
