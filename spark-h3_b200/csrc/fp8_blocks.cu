@@ -112,30 +112,19 @@ __device__ __forceinline__ float swiglu(float a, float g) {
   return a * g * reciprocal(1.f + sm100::ex2_approx(g * -kLog2e));
 }
 
-// x * Phi(x).  For x <= 0, Phi(x) = e^(-x^2 / 2) R(|x|) with R(t) = erfcx(t / sqrt 2) / 2 (half the
-// scaled complementary error function), smooth and without a reciprocal: a degree-11 polynomial on
-// [0, 5.25], fitted here by iteratively reweighted least squares at Chebyshev nodes with weight
-// e^(-t^2 / 2) (1 + t).  Phi is off by at most 1.2e-7 (two steps of fp32 below 1), erff's own
-// spelling 0.5 (1 + erf) by 0.9e-7; R keeps its last value past 5.25, where Phi < 1e-7.
-__device__ __forceinline__ void gelu4(float* x) {
-  constexpr float kR[12] = {0.49999991059303284f,     -0.3989359736442566f,   0.24991749227046967f,
-                            -0.13254864513874054f,    0.061310868710279465f,  -0.024627279490232468f,
-                            0.008287804201245308f,    -0.00220593623816967f,  0.0004333607212174684f,
-                            -5.778570630354807e-05f,  4.603743946063332e-06f, -1.6388463563998812e-07f};
-#pragma unroll
-  for (int i = 0; i < 4; i += 2) {
-    const uint64_t t = sm100::f2_pack(fminf(fabsf(x[i]), 5.25f), fminf(fabsf(x[i + 1]), 5.25f));
-    uint64_t r = sm100::f2_pack(kR[11], kR[11]);
-#pragma unroll
-    for (int k = 10; k >= 0; --k) r = sm100::f2_fma(r, t, sm100::f2_pack(kR[k], kR[k]));
-    const uint64_t xx = sm100::f2_pack(x[i], x[i + 1]);
-    const uint64_t e = sm100::f2_mul(sm100::f2_mul(xx, xx), sm100::f2_pack(-0.5f * kLog2e, -0.5f * kLog2e));
-    float e0, e1, q0, q1;
-    sm100::f2_unpack(e, e0, e1);
-    sm100::f2_unpack(sm100::f2_mul(r, sm100::f2_pack(sm100::ex2_approx(e0), sm100::ex2_approx(e1))), q0, q1);
-    x[i] *= x[i] < 0.f ? q0 : 1.f - q0;
-    x[i + 1] *= x[i + 1] < 0.f ? q1 : 1.f - q1;
-  }
+// x * Phi(x), with Phi(-|x|) from Abramowitz and Stegun 26.2.17 (error below 7.5e-8, as that of
+// erff's spelling 0.5 (1 + erf)): e^(-x^2 / 2) / sqrt(2 pi) times a degree-5 polynomial in
+// 1 / (1 + 0.2316419 |x|), the factor 1 / sqrt(2 pi) taken into the coefficients.  Two special
+// function units' results and eleven products per value, where erff takes about forty
+// instructions (124992 x 4096: 725 us) and a polynomial without the reciprocal, of degree 11, 482.
+__device__ __forceinline__ float gelu(float x) {
+  constexpr float kInvSqrt2Pi = 0.3989422804014327f;
+  constexpr float b1 = 0.319381530f * kInvSqrt2Pi, b2 = -0.356563782f * kInvSqrt2Pi, b3 = 1.781477937f * kInvSqrt2Pi,
+                  b4 = -1.821255978f * kInvSqrt2Pi, b5 = 1.330274429f * kInvSqrt2Pi;
+  const float t = reciprocal(fmaf(0.2316419f, fabsf(x), 1.f));
+  const float poly = fmaf(fmaf(fmaf(fmaf(b5, t, b4), t, b3), t, b2), t, b1) * t;
+  const float q = sm100::ex2_approx(x * x * (-0.5f * kLog2e)) * poly;
+  return x * (x < 0.f ? q : 1.f - q);
 }
 
 // A warp takes U consecutive groups of a row; `row_warps` (1, 2, 4 or 8) warps of a CTA share a
@@ -167,7 +156,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const T*
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[u][i] = swiglu(v[u][i], w[u][i]);
     } else if (ACT == kGelu) {
-      gelu4(v[u]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[u][i] = gelu(v[u][i]);
     }
     const float scale = group_scale(warp_absmax(absmax4(v[u])));
     if (lane == u) mine = scale;
@@ -193,148 +183,196 @@ struct NormParams {
   float eps;
 };
 
-// R consecutive rows of one sample per CTA of W warps (W = 1: one row per warp, eight to a CTA), V
-// groups of 128 columns per warp and row, all in registers.  Two rows share the loads of gate,
-// weight and shift, which outweigh a row's own bytes.  The sum is rounded once, where it is
+// Four elements as loaded, unconverted.
+template <typename T> struct Raw4;
+template <> struct Raw4<__nv_bfloat16> {
+  uint2 r;
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int cols, bool vec) {
+    r = make_uint2(0u, 0u);
+    if (vec) {
+      if (c < cols) r = *reinterpret_cast<const uint2*>(row + c);
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+      if (c + 0 < cols) r.x = h[c];
+      if (c + 1 < cols) r.x |= (uint32_t)h[c + 1] << 16;
+      if (c + 2 < cols) r.y = h[c + 2];
+      if (c + 3 < cols) r.y |= (uint32_t)h[c + 3] << 16;
+    }
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    v[0] = __uint_as_float(r.x << 16);
+    v[1] = __uint_as_float(r.x & 0xffff0000u);
+    v[2] = __uint_as_float(r.y << 16);
+    v[3] = __uint_as_float(r.y & 0xffff0000u);
+  }
+};
+template <> struct Raw4<float> {
+  float r[4];
+  __device__ __forceinline__ void load(const float* row, int c, int cols, bool vec) { load_cols(row, c, cols, vec, r); }
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = r[i];
+  }
+};
+
+constexpr int norm_threads(int W) { return 32 * (W == 1 ? 8 : W); }
+// Rows up to 8192 columns (V <= 4) keep their columns of the parameter vectors in registers.
+constexpr bool norm_keeps(int V) { return V <= 4; }
+constexpr int norm_ctas(int W, int V) { return (V == 4 ? 512 : 768) / norm_threads(W); }  // per SM
+
+// W warps per row (W = 1: eight rows per CTA), V groups of 128 columns per warp, in registers.  CTAs
+// stay and walk the rows with DEPTH further rows in flight (unconverted): a row's work has two or
+// three dependent phases, and loads issued only between them leave HBM idle, as do parameter
+// loads that miss L1 because the rows stream through it.  The sum is rounded once, where it is
 // stored; the norm works on the unrounded fp32 sum.
-template <typename T, int W, int V, int R, bool BLOCKS>
-__global__ void __launch_bounds__(32 * (W == 1 ? 8 : W)) add_rms_norm_quantize_kernel(NormParams p) {
-  __shared__ float red[2][R][W];
+template <typename T, int W, int V, int DEPTH, bool BLOCKS>
+__global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm_quantize_kernel(NormParams p) {
+  constexpr bool KEEP = norm_keeps(V);
+  __shared__ float red[2][2][W];  // [row parity][sum, maximum][warp]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = W == 1 ? 0 : warp;
-  const int64_t row0 = W == 1 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x * R;
-  if (W == 1 && row0 >= p.M) return;  // whole warps leave
-  const int rows = R == 1 ? 1 : (int)min((int64_t)R, p.M - row0);
-  const int64_t sample = p.rows_per_sample == p.M ? 0 : (uint32_t)row0 / (uint32_t)p.rows_per_sample;
-  const T* x = static_cast<const T*>(p.x) + row0 * p.x_stride;
-  float v[R][V][4];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int c = (j * W + part) * kGroup + lane * 4;
-#pragma unroll
-    for (int r = 0; r < R; ++r) load_cols(x + (r < rows ? r : 0) * p.x_stride, c, p.C, p.vec, v[r][j]);
-  }
-  float ss[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) ss[r] = 0.f;
-  if (p.residual != nullptr) {
-    const T* res = static_cast<const T*>(p.residual) + row0 * p.residual_stride;
-    const float* gate = p.gate != nullptr ? p.gate + sample * p.gate_stride : nullptr;
-    T* sum = static_cast<T*>(p.summed) + row0 * p.C;
+  const int c0 = part * kGroup + lane * 4;  // + j * W * kGroup
+  const int64_t step = W == 1 ? (int64_t)gridDim.x * 8 : gridDim.x;
+  const int64_t first = W == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
+  const T* x = static_cast<const T*>(p.x);
+  const T* res = static_cast<const T*>(p.residual);
+  Raw4<T> xr[DEPTH][V], rr[DEPTH][V];
+  auto fetch = [&](int64_t at, Raw4<T>(&xs)[V], Raw4<T>(&rs)[V]) {
+    if (at >= p.M) return;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (j * W + part) * kGroup + lane * 4;
-      float g[4] = {1.f, 1.f, 1.f, 1.f};
-      if (gate != nullptr) load_cols(gate, c, p.C, p.vec_params, g);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float s[4];
-        load_cols(res + (r < rows ? r : 0) * p.residual_stride, c, p.C, p.vec, s);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[r][j][i] = fmaf(g[i], v[r][j][i], s[i]);
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (r < rows) store_cols(sum + (int64_t)r * p.C, c, p.C, p.vec, v[r][j]);
+      xs[j].load(x + at * p.x_stride, c0 + j * W * kGroup, p.C, p.vec);
+      if (res != nullptr) rs[j].load(res + at * p.residual_stride, c0 + j * W * kGroup, p.C, p.vec);
     }
-  }
+  };
+  auto params = [&](const float* base, int64_t at, int j, float fill, float* v) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
+    for (int i = 0; i < 4; ++i) v[i] = fill;
+    if (base != nullptr) load_cols(base + at, c0 + j * W * kGroup, p.C, p.vec_params, v);
+  };
+  float gate[KEEP ? V : 1][4], weight[KEEP ? V : 1][4], shift[KEEP ? V : 1][4];
+  int64_t sample = -1;
+
+  auto process = [&](int64_t row, int parity, Raw4<T>(&xs)[V], Raw4<T>(&rs)[V]) {
+    const int64_t now = p.rows_per_sample == p.M ? 0 : (uint32_t)row / (uint32_t)p.rows_per_sample;
+    if (KEEP && now != sample) {
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss[r] = fmaf(v[r][j][i], v[r][j][i], ss[r]);
-    ss[r] = warp_sum(ss[r]);
-    if (W > 1 && lane == 0) red[0][r][part] = ss[r];
-  }
-  if (W > 1) {
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      ss[r] = red[0][r][0];
-#pragma unroll
-      for (int i = 1; i < W; ++i) ss[r] += red[0][r][i];
-    }
-  }
-  float rstd[R], amax[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    rstd[r] = rsqrtf(ss[r] / (float)p.C + p.eps);
-    amax[r] = 0.f;
-  }
-  const float* weight = p.weight != nullptr ? p.weight + sample * p.weight_stride : nullptr;
-  const float* shift = p.shift != nullptr ? p.shift + sample * p.shift_stride : nullptr;
-  uint8_t* out = p.out + row0 * p.C;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int kb = j * W + part, c = kb * kGroup + lane * 4;
-    float w[4] = {1.f, 1.f, 1.f, 1.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (weight != nullptr) load_cols(weight, c, p.C, p.vec_params, w);
-    if (shift != nullptr) load_cols(shift, c, p.C, p.vec_params, b);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[r][j][i] = fmaf(v[r][j][i] * rstd[r], w[i], b[i]);
-      // Columns past the end stay out of the maximum: their value is 0 unless rstd is not finite
-      // (w and b read as 0 there), and then the whole row is NaN or 0 already.
-      const float m = absmax4(v[r][j]);
-      if (BLOCKS) {
-        const float scale = group_scale(warp_absmax(m));
-        if (r < rows) {
-          if (lane == 0 && kb < p.groups) p.scales[(row0 + r) * p.groups + kb] = scale;
-          store_codes(out + (int64_t)r * p.C, c, p.C, p.vec, v[r][j], reciprocal(scale));
-        }
-      } else {
-        amax[r] = max_nan(amax[r], m);
+      for (int j = 0; j < (KEEP ? V : 1); ++j) {
+        params(p.gate, now * p.gate_stride, j, 1.f, gate[j]);
+        params(p.weight, now * p.weight_stride, j, 1.f, weight[j]);
+        params(p.shift, now * p.shift_stride, j, 0.f, shift[j]);
       }
     }
-  }
-  if (!BLOCKS) {
+    sample = now;
+    float v[V][4];
+    float ss = 0.f;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      amax[r] = warp_absmax(amax[r]);
-      if (W > 1 && lane == 0) red[1][r][part] = amax[r];
-    }
-    if (W > 1) __syncthreads();
+    for (int j = 0; j < V; ++j) {
+      xs[j].get(v[j]);
+      if (res != nullptr) {
+        float s[4], g[4];
+        if (!KEEP) params(p.gate, now * p.gate_stride, j, 1.f, g);
+        rs[j].get(s);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (W > 1) {
-        amax[r] = red[1][r][0];
-#pragma unroll
-        for (int i = 1; i < W; ++i) amax[r] = max_nan(amax[r], red[1][r][i]);
+        for (int i = 0; i < 4; ++i) v[j][i] = fmaf(KEEP ? gate[KEEP ? j : 0][i] : g[i], v[j][i], s[i]);
       }
-      if (r >= rows) continue;
-      const float scale = group_scale(amax[r]);
-      if (part == 0 && lane == 0) p.scales[row0 + r] = scale;
-      const float inv = reciprocal(scale);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss = fmaf(v[j][i], v[j][i], ss);
+    }
+    fetch(row + DEPTH * step, xs, rs);
+    if (res != nullptr) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        store_codes(out + (int64_t)r * p.C, (j * W + part) * kGroup + lane * 4, p.C, p.vec, v[r][j], inv);
+        store_cols(static_cast<T*>(p.summed) + row * p.C, c0 + j * W * kGroup, p.C, p.vec, v[j]);
     }
+    ss = warp_sum(ss);
+    if (W > 1) {
+      if (lane == 0) red[parity][0][part] = ss;
+      __syncthreads();  // also separates this row's use of red from the one two rows ago
+      ss = red[parity][0][0];
+#pragma unroll
+      for (int i = 1; i < W; ++i) ss += red[parity][0][i];
+    }
+    const float rstd = rsqrtf(ss / (float)p.C + p.eps);
+    float amax = 0.f;
+    uint8_t* out = p.out + row * p.C;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int kb = j * W + part;
+      float w[4], b[4];
+      if (!KEEP) {
+        params(p.weight, now * p.weight_stride, j, 1.f, w);
+        params(p.shift, now * p.shift_stride, j, 0.f, b);
+      }
+      // Columns past the end hold 0 * rstd (and a shift of 0), which adds nothing to the maximum:
+      // rstd is NaN only where the row's values are too.
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[j][i] = fmaf(v[j][i] * rstd, KEEP ? weight[KEEP ? j : 0][i] : w[i], KEEP ? shift[KEEP ? j : 0][i] : b[i]);
+      const float m = absmax4(v[j]);
+      if (BLOCKS) {
+        const float scale = group_scale(warp_absmax(m));
+        if (lane == 0 && kb < p.groups) p.scales[row * p.groups + kb] = scale;
+        store_codes(out, c0 + j * W * kGroup, p.C, p.vec, v[j], reciprocal(scale));
+      } else {
+        amax = max_nan(amax, m);
+      }
+    }
+    if (!BLOCKS) {
+      amax = warp_absmax(amax);
+      if (W > 1) {
+        if (lane == 0) red[parity][1][part] = amax;
+        __syncthreads();
+        amax = red[parity][1][0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) amax = max_nan(amax, red[parity][1][i]);
+      }
+      const float scale = group_scale(amax);
+      if (part == 0 && lane == 0) p.scales[row] = scale;
+      const float inv = reciprocal(scale);
+#pragma unroll
+      for (int j = 0; j < V; ++j) store_codes(out, c0 + j * W * kGroup, p.C, p.vec, v[j], inv);
+    }
+  };
+
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) fetch(first + d * step, xr[d], rr[d]);
+  for (int64_t row = first; row < p.M; row += 2 * step) {
+    process(row, 0, xr[0], rr[0]);
+    if (row + step < p.M) process(row + step, 1, xr[DEPTH - 1], rr[DEPTH - 1]);
   }
 }
 
-template <typename T, int W, int V, int R>
+int sm_count() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+template <typename T, int W, int V>
 void launch_norm(const NormParams& p, bool blocks, cudaStream_t s) {
-  const unsigned grid = (unsigned)(W == 1 ? (p.M + 7) / 8 : (p.M + R - 1) / R);
+  // Two rows in flight where their unconverted columns take few registers.
+  constexpr int kDepth = sizeof(T) == 2 && norm_keeps(V) && W > 1 ? 2 : 1;
+  const int64_t ctas = W == 1 ? (p.M + 7) / 8 : p.M, resident = (int64_t)sm_count() * norm_ctas(W, V);
+  const unsigned grid = (unsigned)(ctas < resident ? ctas : resident);
   if (blocks)
-    add_rms_norm_quantize_kernel<T, W, V, R, true><<<grid, 32 * (W == 1 ? 8 : W), 0, s>>>(p);
+    add_rms_norm_quantize_kernel<T, W, V, kDepth, true><<<grid, norm_threads(W), 0, s>>>(p);
   else
-    add_rms_norm_quantize_kernel<T, W, V, R, false><<<grid, 32 * (W == 1 ? 8 : W), 0, s>>>(p);
+    add_rms_norm_quantize_kernel<T, W, V, kDepth, false><<<grid, norm_threads(W), 0, s>>>(p);
 }
 
 template <typename T>
 void dispatch_norm(const NormParams& p, bool blocks, cudaStream_t s) {
-  // Two rows per CTA where they belong to one sample and leave enough CTAs to fill the GPU.
-  const bool two = p.rows_per_sample % 2 == 0 && p.M >= 4096;
-  if (p.C <= 128) return launch_norm<T, 1, 1, 1>(p, blocks, s);
-  if (p.C <= 256) return launch_norm<T, 1, 2, 1>(p, blocks, s);
-  if (p.C <= 512) return launch_norm<T, 1, 4, 1>(p, blocks, s);
-  if (p.C <= 1024 && p.M >= 4096) return launch_norm<T, 1, 8, 1>(p, blocks, s);
-  if (p.C <= 2048) return two ? launch_norm<T, 4, 4, 2>(p, blocks, s) : launch_norm<T, 8, 2, 1>(p, blocks, s);
-  if (p.C <= 4096) return two ? launch_norm<T, 8, 4, 2>(p, blocks, s) : launch_norm<T, 8, 4, 1>(p, blocks, s);
-  if (p.C <= 8192) return two ? launch_norm<T, 16, 4, 2>(p, blocks, s) : launch_norm<T, 16, 4, 1>(p, blocks, s);
-  return launch_norm<T, 16, 8, 1>(p, blocks, s);
+  if (p.C <= 128) return launch_norm<T, 1, 1>(p, blocks, s);
+  if (p.C <= 256) return launch_norm<T, 1, 2>(p, blocks, s);
+  if (p.C <= 512) return launch_norm<T, 1, 4>(p, blocks, s);
+  if (p.C <= 1024) return launch_norm<T, 4, 2>(p, blocks, s);
+  if (p.C <= 2048) return launch_norm<T, 8, 2>(p, blocks, s);
+  if (p.C <= 4096) return launch_norm<T, 8, 4>(p, blocks, s);
+  if (p.C <= 6144) return launch_norm<T, 12, 4>(p, blocks, s);
+  if (p.C <= 8192) return launch_norm<T, 16, 4>(p, blocks, s);
+  return launch_norm<T, 24, 6>(p, blocks, s);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }

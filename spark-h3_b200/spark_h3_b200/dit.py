@@ -4,7 +4,7 @@ one node with a sequence-to-head all-to-all around attention (Ulysses style).
 The reference has no such model on its attention path (its DiT is diffusers' MiniMax-H3); the
 stack here is the minimal block BASELINE names: hidden 4096, 32 heads of 128, GELU FFN 16384,
 RMSNorm, 3-D RoPE over (t, h, w), adaLN timestep modulation, e4m3 linears (per-token x
-per-channel scales), random-init weights N(0, 0.02).  Per block and rank (Nloc = N / P
+per-channel scales, or block scales: linear_scales="block"), random-init weights N(0, 0.02).  Per block and rank (Nloc = N / P
 tokens, P ranks):
 
     x  ->  norm + modulate + quantise  ->  fused QKV GEMM  ->  q/k RMSNorm + RoPE
@@ -26,7 +26,8 @@ import torch.distributed as dist
 import torch.nn.functional as F
 
 from . import _lib
-from .fp8_linear import FP8_DTYPE, fp8_gemm, quantize_weight
+from .fp8_linear import (FP8_DTYPE, add_rms_norm_quantize, fp8_gemm, fp8_gemm_blocks, gelu_quantize_blocks,
+                         quantize_blocks, quantize_weight, quantize_weight_blocks)
 from .ops import _stream
 
 
@@ -169,11 +170,16 @@ class DiTStack:
 
     def __init__(self, cfg: DiTConfig, grid, *, device, world: int = 1, rank: int = 0, group=None, seed: int = 0,
                  spark_mode: str = "full", topk_ratio: float = 0.1, steps: int = 19, fused_producer: bool = True,
-                 peer_exchange: bool = False):
+                 peer_exchange: bool = False, linear_scales: str = "channel"):
         from .config import H3SparseAttentionConfig
         from .layout import PackedLayout
         from .processor import _Controller
 
+        if linear_scales not in ("channel", "block"):
+            raise ValueError(f'linear_scales must be "channel" or "block", got {linear_scales!r}')
+        self.block_scales = linear_scales == "block"
+        if self.block_scales and peer_exchange:
+            raise ValueError("peer_exchange belongs to the per-channel producer; block scales exchange through NCCL")
         self.cfg, self.grid, self.device = cfg, tuple(grid), torch.device(device)
         self.world, self.rank, self.group = world, rank, group
         self.tokens = grid[0] * grid[1] * grid[2]
@@ -186,7 +192,7 @@ class DiTStack:
 
         def linear(out_f, in_f):
             w = (torch.randn(out_f, in_f, device=self.device, generator=g) * 0.02).to(torch.bfloat16)
-            return quantize_weight(w)
+            return quantize_weight_blocks(w) if self.block_scales else quantize_weight(w)
 
         self.blocks = []
         for _ in range(cfg.blocks):
@@ -198,7 +204,7 @@ class DiTStack:
         self.inv_freq, self.axis = rope_tables(cfg, self.device)
         self.coords = token_coords(self.grid, rank * self.local, self.local, self.device)
         # (cos, sin) of every pair and coordinate value, for the GEMM-epilogue producer
-        self.fused_producer = fused_producer and cfg.heads % 2 == 0
+        self.fused_producer = fused_producer and cfg.heads % 2 == 0 and not self.block_scales
         self.rope_stride = max(self.grid)
         ang = torch.arange(self.rope_stride, device=self.device, dtype=torch.float32)[None, :] * self.inv_freq[:, None]
         self.rope = torch.stack((torch.cos(ang), torch.sin(ang)), dim=-1).contiguous()  # [D/2, stride, 2]
@@ -317,6 +323,33 @@ class DiTStack:
 
         return timed()
 
+    def _block_scaled(self, x, blk, mod, layer: int, dense: bool):
+        """One block with block-scaled linears: the attention branch's gated residual is added by
+        the second norm (add_rms_norm_quantize), the feed-forward's by the down projection."""
+        cfg = self.cfg
+        shift1, scale1, gate1, shift2, scale2, gate2 = mod
+        hq, hs, _ = add_rms_norm_quantize(x, 1 + scale1, shift=shift1, eps=cfg.eps)
+        q, k, v = self._qkv_rope(fp8_gemm_blocks(hq, hs, *blk["qkv"]), blk)
+        with self._exchange():
+            qh, kh, vh = (exchange_to_heads(t_, self.group).unsqueeze(0) for t_ in (q, k, v))
+        del q, k, v
+        o = self._attention(qh, kh, vh, layer, dense)
+        del qh, kh, vh
+        with self._exchange():
+            o_seg = exchange_to_tokens(o[0], self.world, self.group)
+        # o_seg [P, Nloc, Hp, D]: heads are 128 wide, so each segment quantises on its own; the
+        # codes and scales, not the activation, are put in row order.
+        oq, os_ = quantize_blocks(o_seg.view(self.world * self.local, -1))
+        oq, os_ = (t_.view(self.world, self.local, -1).transpose(0, 1).reshape(self.local, -1) for t_ in (oq, os_))
+        del o_seg
+        delta = fp8_gemm_blocks(oq, os_, *blk["out"])
+        hq, hs, _ = add_rms_norm_quantize(delta, 1 + scale2, x, gate=gate1, shift=shift2, eps=cfg.eps, out=x)
+        del delta
+        f = fp8_gemm_blocks(hq, hs, *blk["up"])
+        fq, fs = gelu_quantize_blocks(f)
+        del f
+        fp8_gemm_blocks(fq, fs, *blk["down"], residual=x, gate=gate2, out=x)
+
     def modulation(self, t: float):
         temb = F.silu(timestep_embedding(t, self.cfg.t_dim, self.device))
         return [(blk["ada"] @ temb).view(6, self.cfg.hidden).contiguous() for blk in self.blocks]
@@ -328,6 +361,9 @@ class DiTStack:
             raise ValueError(f"x must be contiguous bf16 [{self.local}, {self.cfg.hidden}]")
         for layer, (blk, mod) in enumerate(zip(self.blocks, self.modulation(t))):
             shift1, scale1, gate1, shift2, scale2, gate2 = mod
+            if self.block_scales:
+                self._block_scaled(x, blk, mod, layer, dense)
+                continue
             hq, hs = self._norm_quant(x, shift1, scale1)
             if self.peer is not None:
                 self._qkv_producer_peers(hq, hs, blk)
@@ -358,15 +394,23 @@ class DiTStack:
         return x
 
 
-def reference_block_math(x, blk, mod, cfg: DiTConfig, coords, inv_freq, axis, attention):
+def reference_block_math(x, blk, mod, cfg: DiTConfig, coords, inv_freq, axis, attention, linear_scales="channel"):
     """fp32 torch restatement of one block on one rank (P = 1) with the same e4m3 activation
     and weight quantisation, for the tests."""
-    from .fp8_linear import quantize_rows_reference
+    from .fp8_linear import quantize_blocks_reference, quantize_rows_reference
+
+    def spread(s, n):
+        return s.repeat_interleave(128, dim=-1)[..., :n]
 
     def deq(w):
+        if linear_scales == "block":
+            return w[0].float() * spread(spread(w[1], w[0].shape[1]).T, w[0].shape[0]).T
         return w[0].float() * w[1].reshape(-1, 1)
 
     def lin(h, w):
+        if linear_scales == "block":
+            hq, hs = quantize_blocks_reference(h)
+            return (hq.float() * spread(hs, h.shape[1])) @ deq(w).T
         hq, hs = quantize_rows_reference(h)
         return (hq.float() * hs) @ deq(w).T
 

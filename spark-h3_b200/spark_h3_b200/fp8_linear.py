@@ -131,10 +131,11 @@ def _strided_rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, i
     return x, M, C, stride if M > 1 else C
 
 
-def _same_device(device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise RuntimeError(f"all tensors must be on the same CUDA device: {name} is on {t.device}, not {device}")
+def _same_device(device: torch.device, *tensors) -> None:
+    index = device.index
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"all tensors must be on the same CUDA device: one is on {t.device}, not {device}")
 
 
 def _call_on(device: torch.device, name: str, *args) -> None:
@@ -173,6 +174,14 @@ def quantize_blocks(x: torch.Tensor):
     return _quantize_blocks("sb_fp8_quantize_blocks", x, 1)
 
 
+def quantize_blocks_reference(x: torch.Tensor):
+    """The eager spelling of quantize_blocks, for the tests."""
+    M, K = x.shape
+    y = F.pad(x.float(), (0, _blocks(K) * BLOCK - K)).view(M, -1, BLOCK)
+    scale = (y.abs().amax(dim=2) / FP8_MAX).clamp_min(1e-12)
+    return (y / scale[:, :, None]).to(FP8_DTYPE).view(M, -1)[:, :K], scale
+
+
 def swiglu_quantize_blocks(h: torch.Tensor):
     """[M, 2K] projection output -> quantize_blocks(a * silu(gate)) with a, gate = h.chunk(2),
     without writing the activation."""
@@ -184,20 +193,18 @@ def gelu_quantize_blocks(x: torch.Tensor):
     return _quantize_blocks("sb_fp8_gelu_quantize_blocks", x, 1)
 
 
-def _sample_vector(v: torch.Tensor | None, name: str, M: int, C: int, samples: int):
+def _sample_vector(v: torch.Tensor, name: str, M: int, C: int, samples: int):
     """A vector [C] or one per sample [S, C] as (fp32 tensor, stride between samples, S)."""
-    if v is None:
-        return None, 0, samples
-    dims = v.dim()
-    if dims not in (1, 2) or v.shape[-1] != C:
-        raise ValueError(f"{name} must be [{C}] or [samples, {C}], got {tuple(v.shape)}")
+    shape = v.shape
+    if shape[-1:] != (C,) or len(shape) > 2:
+        raise ValueError(f"{name} must be [{C}] or [samples, {C}], got {tuple(shape)}")
     if v.dtype != torch.float32:
         v = v.float()
     if not v.is_contiguous() and v.stride(-1) != 1:
         v = v.contiguous()
-    if dims == 1 or v.shape[0] == 1:
+    if len(shape) == 1 or shape[0] == 1:
         return v, 0, samples
-    S = v.shape[0]
+    S = shape[0]
     if S == 0 or M % S or (samples not in (1, S)):
         raise ValueError(f"{name} has {S} samples: {M} rows must split evenly among one number of samples")
     return v, v.stride(0), S
@@ -229,16 +236,22 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
             out = torch.empty(M, C, device=device, dtype=x.dtype)
         elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {tuple(x.shape)} {x.dtype}")
-    _same_device(device, residual=residual, weight=weight, gate=gate, shift=shift, out=out)
-    samples = 1
-    gate, g_stride, samples = _sample_vector(gate, "gate", M, C, samples)
-    weight, w_stride, samples = _sample_vector(weight, "weight", M, C, samples)
-    shift, s_stride, samples = _sample_vector(shift, "shift", M, C, samples)
+    _same_device(device, residual, weight, gate, shift, out)
+    samples, gate_ptr, g_stride, weight_ptr, w_stride, shift_ptr, s_stride = 1, None, 0, None, 0, None, 0
+    if gate is not None:
+        gate, g_stride, samples = _sample_vector(gate, "gate", M, C, samples)
+        gate_ptr = gate.data_ptr()
+    if weight is not None:
+        weight, w_stride, samples = _sample_vector(weight, "weight", M, C, samples)
+        weight_ptr = weight.data_ptr()
+    if shift is not None:
+        shift, s_stride, samples = _sample_vector(shift, "shift", M, C, samples)
+        shift_ptr = shift.data_ptr()
     y = torch.empty(M, C, device=device, dtype=FP8_DTYPE)
     scale = torch.empty(M, _blocks(C) if blocks else 1, device=device, dtype=torch.float32)
     if M > 0:
-        _call_on(device, "sb_fp8_add_rms_norm_quantize", x.data_ptr(), x_stride, _ptr(residual), r_stride, _ptr(gate),
-                 g_stride, _ptr(weight), w_stride, _ptr(shift), s_stride, dtype, M, C, M // samples, eps, int(blocks),
+        _call_on(device, "sb_fp8_add_rms_norm_quantize", x.data_ptr(), x_stride, _ptr(residual), r_stride, gate_ptr,
+                 g_stride, weight_ptr, w_stride, shift_ptr, s_stride, dtype, M, C, M // samples, eps, 1 if blocks else 0,
                  _ptr(out), y.data_ptr(), scale.data_ptr())
     return y, scale, out
 
@@ -258,14 +271,16 @@ def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Ten
     if not a_fp8.is_cuda:
         raise RuntimeError("spark_h3_b200 kernels require CUDA tensors; there is no CPU path")
     device = a_fp8.device
-    _same_device(device, a_scale=a_scale, b_fp8=b_fp8, b_scale=b_scale, bias=bias, residual=residual, gate=gate, out=out)
+    _same_device(device, a_scale, b_fp8, b_scale, bias, residual, gate, out)
     a_fp8, b_fp8, b_scale = a_fp8.contiguous(), b_fp8.contiguous(), b_scale.contiguous()
     (M, K), N = a_fp8.shape, b_fp8.shape[0]
-    for scale, rows, name in ((a_scale, M, "a_scale"), (b_scale, _blocks(N), "b_scale")):
-        if scale.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32")
-        if scale.shape != (rows, _blocks(K)):
-            raise ValueError(f"{name} must be [{rows}, {_blocks(K)}], got {tuple(scale.shape)}")
+    kb = -(-K // BLOCK)
+    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+        raise TypeError(f"{'b' if a_scale.dtype == torch.float32 else 'a'}_scale must be float32")
+    if a_scale.shape != (M, kb):
+        raise ValueError(f"a_scale must be [{M}, {kb}], got {tuple(a_scale.shape)}")
+    if b_scale.shape != (-(-N // BLOCK), kb):
+        raise ValueError(f"b_scale must be [{_blocks(N)}, {kb}], got {tuple(b_scale.shape)}")
     if out is not None:
         out_dtype = out_dtype or out.dtype
     elif out_dtype is None:
@@ -290,8 +305,9 @@ def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Ten
     elif gate is not None:
         raise ValueError("gate belongs to the residual's addition: pass a residual")
     if M > 0 and N > 0:
-        _call_on(device, "sb_fp8_gemm_blocks", a_fp8.data_ptr(), a_scale.data_ptr(), a_scale.stride(0),
-                 a_scale.stride(1), b_fp8.data_ptr(), b_scale.data_ptr(), M, N, K, _ptr(bias), _ptr(residual),
+        row_stride, block_stride = a_scale.stride()
+        _call_on(device, "sb_fp8_gemm_blocks", a_fp8.data_ptr(), a_scale.data_ptr(), row_stride, block_stride,
+                 b_fp8.data_ptr(), b_scale.data_ptr(), M, N, K, _ptr(bias), _ptr(residual),
                  _ptr(gate), out.data_ptr(), code)
     return out
 

@@ -578,3 +578,56 @@ def test_install_with_block_scales(cuda_device):
         assert fl.forward_qkv_shared(attn, x) is None
         attn.to_k = fl.Fp8Linear(attn.to_k)
         assert fl.forward_qkv_shared(attn, x) is None  # another granularity
+
+
+def test_stack_rejects_unknown_linear_scales():
+    from spark_h3_b200.dit import DiTConfig, DiTStack
+
+    cfg = DiTConfig(hidden=256, heads=2, ffn=512, blocks=1)
+    with pytest.raises(ValueError, match="linear_scales"):
+        DiTStack(cfg, (1, 4, 8), device="cpu", linear_scales="tensor")
+    with pytest.raises(ValueError, match="peer_exchange"):
+        DiTStack(cfg, (1, 4, 8), device="cpu", linear_scales="block", peer_exchange=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dense", [True, False])
+def test_stack_step_with_block_scales(cuda_device, dense):
+    """The DiT stack with block-scaled linears against the fp32 restatement of its block, to the
+    bounds of the per-channel stack's own test."""
+    from spark_h3_b200.attention import spark_attention_bthd
+    from spark_h3_b200.dit import DiTConfig, DiTStack, reference_block_math
+
+    cfg = DiTConfig(hidden=256, heads=2, ffn=512, blocks=2)
+    stack = DiTStack(cfg, (2, 16, 32), device=cuda_device, seed=3, spark_mode="reweight_only", topk_ratio=0.2,
+                     linear_scales="block")
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    x0 = torch.randn(stack.local, cfg.hidden, device=cuda_device, generator=g).to(torch.bfloat16)
+    x = stack.step(x0.clone(), 500.0, dense=dense)
+
+    def attention(q, k, v):
+        if dense:
+            o = F.scaled_dot_product_attention(q.float().transpose(1, 2), k.float().transpose(1, 2),
+                                               v.float().transpose(1, 2))
+            return o.transpose(1, 2).to(torch.bfloat16)
+        return spark_attention_bthd(stack.controller, q.contiguous(), k.contiguous(), v.contiguous(), stack.layout, 0)
+
+    ref = x0
+    for blk, mod in zip(stack.blocks, stack.modulation(500.0)):
+        ref = reference_block_math(ref, blk, mod, cfg, stack.coords, stack.inv_freq, stack.axis, attention, "block")
+    diff = (x.float() - ref.float()).abs().max().item()
+    cos = F.cosine_similarity(x.float().flatten(), ref.float().flatten(), dim=0).item()
+    assert torch.isfinite(x).all()
+    assert cos > 0.999 and diff <= 0.05 * ref.float().abs().max().item(), (cos, diff)
+
+
+@pytest.mark.gpu
+def test_attention_segments_quantise_in_row_order(cuda_device):
+    """Codes and scales of two ranks' head segments, put in row order, are those of the rows."""
+    M, hp = 50, 2
+    seg = torch.randn(2, M, hp * 128, device=cuda_device).to(torch.bfloat16)
+    rows = seg.transpose(0, 1).reshape(M, -1)
+    codes, scale = fl.quantize_blocks(seg.view(2 * M, -1))
+    got = tuple(t.view(2, M, -1).transpose(0, 1).reshape(M, -1) for t in (codes, scale))
+    want = fl.quantize_blocks(rows)
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
