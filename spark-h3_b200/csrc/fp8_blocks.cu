@@ -5,8 +5,9 @@
 // A warp holds a group of 128 columns, four consecutive ones per lane, so the group's maximum is
 // one warp-wide reduction instruction.  What bounds these kernels is HBM once the instructions per
 // value are few: at 6.5 TB/s an SM issues about 17 per bf16 value in the time that its three bytes
-// take (the first form, half a warp per group with eight shuffle steps, 64-bit index divisions and
-// exact divisions, took 24 and ran at 4.5 TB/s; GELU with erff took 50).
+// take.  124992 x 4096 bf16: 232 us, 6.6 TB/s (half a warp per group with shuffles, 64-bit index
+// divisions and exact divisions: 341); SwiGLU of 124992 x 2 x 2048: 222 us, 5.8 TB/s; GELU: 444 us,
+// bound by its instructions.
 //
 // Scales and special values follow torch's spelling of the same arithmetic: scale =
 // max(absmax * fp32(1/448), 1e-12) and the maximum propagates NaN, so a NaN in a group makes
@@ -115,8 +116,8 @@ __device__ __forceinline__ float swiglu(float a, float g) {
 // x * Phi(x), with Phi(-|x|) from Abramowitz and Stegun 26.2.17 (error below 7.5e-8, as that of
 // erff's spelling 0.5 (1 + erf)): e^(-x^2 / 2) / sqrt(2 pi) times a degree-5 polynomial in
 // 1 / (1 + 0.2316419 |x|), the factor 1 / sqrt(2 pi) taken into the coefficients.  Two special
-// function units' results and eleven products per value, where erff takes about forty
-// instructions (124992 x 4096: 725 us) and a polynomial without the reciprocal, of degree 11, 482.
+// function units' results and eleven products per value (124992 x 4096: 444 us); erff's spelling
+// takes 725 us, a polynomial of degree 11 without the reciprocal 482.
 __device__ __forceinline__ float gelu(float x) {
   constexpr float kInvSqrt2Pi = 0.3989422804014327f;
   constexpr float b1 = 0.319381530f * kInvSqrt2Pi, b2 = -0.356563782f * kInvSqrt2Pi, b3 = 1.781477937f * kInvSqrt2Pi,
@@ -131,10 +132,10 @@ __device__ __forceinline__ float gelu(float x) {
 // row, blockIdx.y counts further 8 * U groups.
 constexpr int kQuantThreads = 256;
 
-template <typename T, int ACT, int U>
+template <typename T, int ACT, int U, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const T* __restrict__ x, int64_t x_stride,
                                                                         int64_t M, int groups, int K, int row_shift,
-                                                                        int vec, uint8_t* __restrict__ out,
+                                                                        uint8_t* __restrict__ out,
                                                                         float* __restrict__ scales) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = ((int64_t)blockIdx.x << (3 - row_shift)) + (warp >> row_shift);
@@ -146,8 +147,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const T*
   float v[U][4], w[ACT == kSwiglu ? U : 1][4];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    load_cols(xr, c0 + u * kGroup, K, vec, v[u]);
-    if (ACT == kSwiglu) load_cols(xr + K, c0 + u * kGroup, K, vec, w[u]);
+    load_cols(xr, c0 + u * kGroup, K, VEC, v[u]);
+    if (ACT == kSwiglu) load_cols(xr + K, c0 + u * kGroup, K, VEC, w[u]);
   }
   float mine = 0.f;
 #pragma unroll
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const T*
     }
     const float scale = group_scale(warp_absmax(absmax4(v[u])));
     if (lane == u) mine = scale;
-    store_codes(yr, c0 + u * kGroup, K, vec, v[u], reciprocal(scale));
+    store_codes(yr, c0 + u * kGroup, K, VEC, v[u], reciprocal(scale));
   }
   if (lane < U && g0 + lane < groups) scales[row * groups + g0 + lane] = mine;
 }
@@ -179,7 +180,7 @@ struct NormParams {
   int64_t gate_stride, weight_stride, shift_stride;  // floats between samples
   int64_t M, rows_per_sample;
   int C, groups;
-  int vec, vec_params;  // vector accesses to the rows / to the parameter vectors
+  int vec;  // everything is aligned for accesses of four elements
   float eps;
 };
 
@@ -216,130 +217,169 @@ template <> struct Raw4<float> {
 };
 
 constexpr int norm_threads(int W) { return 32 * (W == 1 ? 8 : W); }
-// Rows up to 8192 columns (V <= 4) keep their columns of the parameter vectors in registers.
+// Rows up to 8192 columns (V <= 4) keep their columns of weight and shift in registers.
 constexpr bool norm_keeps(int V) { return V <= 4; }
 constexpr int norm_ctas(int W, int V) { return (V == 4 ? 512 : 768) / norm_threads(W); }  // per SM
 
 // W warps per row (W = 1: eight rows per CTA), V groups of 128 columns per warp, in registers.  CTAs
-// stay and walk the rows with DEPTH further rows in flight (unconverted): a row's work has two or
-// three dependent phases, and loads issued only between them leave HBM idle, as do parameter
-// loads that miss L1 because the rows stream through it.  The sum is rounded once, where it is
-// stored; the norm works on the unrounded fp32 sum.
-template <typename T, int W, int V, int DEPTH, bool BLOCKS>
+// stay and walk the rows, R at a time: a row's work is a chain (sum over the CTA, then scale, then
+// codes) of about 2000 cycles, so R rows go through it together, the next R rows in flight
+// (unconverted) meanwhile.  The sum is rounded once, where it is stored; the norm works on the
+// unrounded fp32 sum.  Measured at 124992 x 4096 bf16 with residual, gate and shift (3.6 GB): 615 us,
+// 5.8 TB/s; one row at a time 659, one row per CTA without rows in flight 832, access-by-access
+// alignment checks instead of VEC 746.
+template <typename T, int W, int V, int R, bool BLOCKS, bool VEC>
 __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm_quantize_kernel(NormParams p) {
   constexpr bool KEEP = norm_keeps(V);
-  __shared__ float red[2][2][W];  // [row parity][sum, maximum][warp]
+  __shared__ float red[2][2][R][W];  // [parity][sum, maximum][row][warp]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = W == 1 ? 0 : warp;
   const int c0 = part * kGroup + lane * 4;  // + j * W * kGroup
   const int64_t step = W == 1 ? (int64_t)gridDim.x * 8 : gridDim.x;
-  const int64_t first = W == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
+  int64_t row = W == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
   const T* x = static_cast<const T*>(p.x);
   const T* res = static_cast<const T*>(p.residual);
-  Raw4<T> xr[DEPTH][V], rr[DEPTH][V];
-  auto fetch = [&](int64_t at, Raw4<T>(&xs)[V], Raw4<T>(&rs)[V]) {
-    if (at >= p.M) return;
+  Raw4<T> xr[R][V], rr[R][V];
+  auto fetch = [&](int64_t at) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      xs[j].load(x + at * p.x_stride, c0 + j * W * kGroup, p.C, p.vec);
-      if (res != nullptr) rs[j].load(res + at * p.residual_stride, c0 + j * W * kGroup, p.C, p.vec);
+    for (int r = 0; r < R; ++r, at += step) {
+      if (at >= p.M) break;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        xr[r][j].load(x + at * p.x_stride, c0 + j * W * kGroup, p.C, VEC);
+        if (res != nullptr) rr[r][j].load(res + at * p.residual_stride, c0 + j * W * kGroup, p.C, VEC);
+      }
     }
   };
   auto params = [&](const float* base, int64_t at, int j, float fill, float* v) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = fill;
-    if (base != nullptr) load_cols(base + at, c0 + j * W * kGroup, p.C, p.vec_params, v);
+    if (base != nullptr) load_cols(base + at, c0 + j * W * kGroup, p.C, VEC, v);
   };
-  float gate[KEEP ? V : 1][4], weight[KEEP ? V : 1][4], shift[KEEP ? V : 1][4];
-  int64_t sample = -1;
+  auto sample_of = [&](int64_t at) -> int64_t {
+    return p.rows_per_sample == p.M ? 0 : (uint32_t)at / (uint32_t)p.rows_per_sample;
+  };
+  float weight[KEEP ? V : 1][4], shift[KEEP ? V : 1][4];
+  int64_t kept = -1;  // the sample of weight and shift
 
-  auto process = [&](int64_t row, int parity, Raw4<T>(&xs)[V], Raw4<T>(&rs)[V]) {
-    const int64_t now = p.rows_per_sample == p.M ? 0 : (uint32_t)row / (uint32_t)p.rows_per_sample;
-    if (KEEP && now != sample) {
 #pragma unroll
-      for (int j = 0; j < (KEEP ? V : 1); ++j) {
-        params(p.gate, now * p.gate_stride, j, 1.f, gate[j]);
-        params(p.weight, now * p.weight_stride, j, 1.f, weight[j]);
-        params(p.shift, now * p.shift_stride, j, 0.f, shift[j]);
-      }
-    }
-    sample = now;
-    float v[V][4];
-    float ss = 0.f;
+  for (int r = 0; r < R; ++r)  // rows past the end are computed on zeros and not stored
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      xs[j].get(v[j]);
-      if (res != nullptr) {
-        float s[4], g[4];
-        if (!KEEP) params(p.gate, now * p.gate_stride, j, 1.f, g);
-        rs[j].get(s);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[j][i] = fmaf(KEEP ? gate[KEEP ? j : 0][i] : g[i], v[j][i], s[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss = fmaf(v[j][i], v[j][i], ss);
+      xr[r][j] = Raw4<T>{};
+      rr[r][j] = Raw4<T>{};
     }
-    fetch(row + DEPTH * step, xs, rs);
+  if (row < p.M) fetch(row);
+  for (int parity = 0; row < p.M; row += R * step, parity ^= 1) {
+    float v[R][V][4], ss[R], rstd[R], amax[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t at = row + r * step;
+      const float* gate = p.gate == nullptr ? nullptr : p.gate + sample_of(at) * p.gate_stride;
+      ss[r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        xr[r][j].get(v[r][j]);
+        if (res != nullptr) {
+          float s[4], g[4];
+          params(at < p.M ? gate : nullptr, 0, j, 1.f, g);
+          rr[r][j].get(s);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[r][j][i] = fmaf(g[i], v[r][j][i], s[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss[r] = fmaf(v[r][j][i], v[r][j][i], ss[r]);
+      }
+    }
+    fetch(row + R * step);
     if (res != nullptr) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        store_cols(static_cast<T*>(p.summed) + row * p.C, c0 + j * W * kGroup, p.C, p.vec, v[j]);
+      for (int r = 0; r < R; ++r)
+        if (row + r * step < p.M) {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            store_cols(static_cast<T*>(p.summed) + (row + r * step) * p.C, c0 + j * W * kGroup, p.C, VEC, v[r][j]);
+        }
     }
-    ss = warp_sum(ss);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      ss[r] = warp_sum(ss[r]);
+      if (W > 1 && lane == 0) red[parity][0][r][part] = ss[r];
+    }
     if (W > 1) {
-      if (lane == 0) red[parity][0][part] = ss;
-      __syncthreads();  // also separates this row's use of red from the one two rows ago
-      ss = red[parity][0][0];
+      __syncthreads();  // also separates this use of red from the one two rounds ago
 #pragma unroll
-      for (int i = 1; i < W; ++i) ss += red[parity][0][i];
-    }
-    const float rstd = rsqrtf(ss / (float)p.C + p.eps);
-    float amax = 0.f;
-    uint8_t* out = p.out + row * p.C;
+      for (int r = 0; r < R; ++r) {
+        ss[r] = red[parity][0][r][0];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int kb = j * W + part;
-      float w[4], b[4];
-      if (!KEEP) {
-        params(p.weight, now * p.weight_stride, j, 1.f, w);
-        params(p.shift, now * p.shift_stride, j, 0.f, b);
+        for (int i = 1; i < W; ++i) ss[r] += red[parity][0][r][i];
       }
-      // Columns past the end hold 0 * rstd (and a shift of 0), which adds nothing to the maximum:
-      // rstd is NaN only where the row's values are too.
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[j][i] = fmaf(v[j][i] * rstd, KEEP ? weight[KEEP ? j : 0][i] : w[i], KEEP ? shift[KEEP ? j : 0][i] : b[i]);
-      const float m = absmax4(v[j]);
-      if (BLOCKS) {
-        const float scale = group_scale(warp_absmax(m));
-        if (lane == 0 && kb < p.groups) p.scales[row * p.groups + kb] = scale;
-        store_codes(out, c0 + j * W * kGroup, p.C, p.vec, v[j], reciprocal(scale));
-      } else {
-        amax = max_nan(amax, m);
+    for (int r = 0; r < R; ++r) {
+      rstd[r] = rsqrtf(ss[r] / (float)p.C + p.eps);
+      amax[r] = 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t at = row + r * step;
+      if (at >= p.M) break;
+      const int64_t sample = sample_of(at);
+      if (KEEP && sample != kept) {
+#pragma unroll
+        for (int j = 0; j < (KEEP ? V : 1); ++j) {
+          params(p.weight, sample * p.weight_stride, j, 1.f, weight[j]);
+          params(p.shift, sample * p.shift_stride, j, 0.f, shift[j]);
+        }
+      }
+      kept = sample;
+      uint8_t* out = p.out + at * p.C;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int kb = j * W + part;
+        float w[4], b[4];
+        if (!KEEP) {
+          params(p.weight, sample * p.weight_stride, j, 1.f, w);
+          params(p.shift, sample * p.shift_stride, j, 0.f, b);
+        }
+        // Columns past the end hold 0 * rstd (and a shift of 0), which adds nothing to the
+        // maximum: rstd is NaN only where the row's values are too.
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[r][j][i] = fmaf(v[r][j][i] * rstd[r], KEEP ? weight[KEEP ? j : 0][i] : w[i], KEEP ? shift[KEEP ? j : 0][i] : b[i]);
+        const float m = absmax4(v[r][j]);
+        if (BLOCKS) {
+          const float scale = group_scale(warp_absmax(m));
+          if (lane == 0 && kb < p.groups) p.scales[at * p.groups + kb] = scale;
+          store_codes(out, c0 + j * W * kGroup, p.C, VEC, v[r][j], reciprocal(scale));
+        } else {
+          amax[r] = max_nan(amax[r], m);
+        }
       }
     }
     if (!BLOCKS) {
-      amax = warp_absmax(amax);
-      if (W > 1) {
-        if (lane == 0) red[parity][1][part] = amax;
-        __syncthreads();
-        amax = red[parity][1][0];
 #pragma unroll
-        for (int i = 1; i < W; ++i) amax = max_nan(amax, red[parity][1][i]);
+      for (int r = 0; r < R; ++r) {
+        amax[r] = warp_absmax(amax[r]);
+        if (W > 1 && lane == 0) red[parity][1][r][part] = amax[r];
       }
-      const float scale = group_scale(amax);
-      if (part == 0 && lane == 0) p.scales[row] = scale;
-      const float inv = reciprocal(scale);
+      if (W > 1) __syncthreads();
 #pragma unroll
-      for (int j = 0; j < V; ++j) store_codes(out, c0 + j * W * kGroup, p.C, p.vec, v[j], inv);
+      for (int r = 0; r < R; ++r) {
+        const int64_t at = row + r * step;
+        if (at >= p.M) break;
+        if (W > 1) {
+          amax[r] = red[parity][1][r][0];
+#pragma unroll
+          for (int i = 1; i < W; ++i) amax[r] = max_nan(amax[r], red[parity][1][r][i]);
+        }
+        const float scale = group_scale(amax[r]);
+        if (part == 0 && lane == 0) p.scales[at] = scale;
+        const float inv = reciprocal(scale);
+#pragma unroll
+        for (int j = 0; j < V; ++j) store_codes(p.out + at * p.C, c0 + j * W * kGroup, p.C, VEC, v[r][j], inv);
+      }
     }
-  };
-
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d) fetch(first + d * step, xr[d], rr[d]);
-  for (int64_t row = first; row < p.M; row += 2 * step) {
-    process(row, 0, xr[0], rr[0]);
-    if (row + step < p.M) process(row + step, 1, xr[DEPTH - 1], rr[DEPTH - 1]);
   }
 }
 
@@ -352,14 +392,15 @@ int sm_count() {
 
 template <typename T, int W, int V>
 void launch_norm(const NormParams& p, bool blocks, cudaStream_t s) {
-  // Two rows in flight where their unconverted columns take few registers.
-  constexpr int kDepth = sizeof(T) == 2 && norm_keeps(V) && W > 1 ? 2 : 1;
+  // Two rows at a time where their unconverted columns take few registers.
+  constexpr int kTogether = sizeof(T) == 2 && norm_keeps(V) && W > 1 ? 2 : 1;
   const int64_t ctas = W == 1 ? (p.M + 7) / 8 : p.M, resident = (int64_t)sm_count() * norm_ctas(W, V);
   const unsigned grid = (unsigned)(ctas < resident ? ctas : resident);
-  if (blocks)
-    add_rms_norm_quantize_kernel<T, W, V, kDepth, true><<<grid, norm_threads(W), 0, s>>>(p);
-  else
-    add_rms_norm_quantize_kernel<T, W, V, kDepth, false><<<grid, norm_threads(W), 0, s>>>(p);
+  auto kernel = blocks ? (p.vec ? add_rms_norm_quantize_kernel<T, W, V, kTogether, true, true>
+                                : add_rms_norm_quantize_kernel<T, W, V, kTogether, true, false>)
+                       : (p.vec ? add_rms_norm_quantize_kernel<T, W, V, kTogether, false, true>
+                                : add_rms_norm_quantize_kernel<T, W, V, kTogether, false, false>);
+  kernel<<<grid, norm_threads(W), 0, s>>>(p);
 }
 
 template <typename T>
@@ -390,7 +431,7 @@ int quantize_blocks(const char* what, const void* x, int64_t x_stride, int dtype
                what);
   const int groups = ceil_div(K, kGroup);
   // Vector accesses need every row (and the gate half) on a boundary of four elements.
-  const int vec = K % 4 == 0 && x_stride % 4 == 0 && (uintptr_t)x % (4 * size) == 0 && (uintptr_t)out % 4 == 0;
+  const bool vec = K % 4 == 0 && x_stride % 4 == 0 && (uintptr_t)x % (4 * size) == 0 && (uintptr_t)out % 4 == 0;
   cudaStream_t s = (cudaStream_t)stream;
   // Few rows: one group per warp, for the most warps; otherwise four loads in flight per lane.
   const bool four = groups >= 4 && M * groups >= 4096;
@@ -399,23 +440,16 @@ int quantize_blocks(const char* what, const void* x, int64_t x_stride, int dtype
   while (row_shift < 3 && (1 << row_shift) < parts) ++row_shift;
   const int rows = 8 >> row_shift;
   const dim3 grid((unsigned)((M + rows - 1) / rows), (unsigned)ceil_div(parts, 8));
-  if (dtype == SB_BF16) {
-    const __nv_bfloat16* h = (const __nv_bfloat16*)x;
-    if (four)
-      quantize_blocks_kernel<__nv_bfloat16, ACT, 4>
-          <<<grid, kQuantThreads, 0, s>>>(h, x_stride, M, groups, K, row_shift, vec, out, scales);
-    else
-      quantize_blocks_kernel<__nv_bfloat16, ACT, 1>
-          <<<grid, kQuantThreads, 0, s>>>(h, x_stride, M, groups, K, row_shift, vec, out, scales);
-  } else {
-    const float* f = (const float*)x;
-    if (four)
-      quantize_blocks_kernel<float, ACT, 4>
-          <<<grid, kQuantThreads, 0, s>>>(f, x_stride, M, groups, K, row_shift, vec, out, scales);
-    else
-      quantize_blocks_kernel<float, ACT, 1>
-          <<<grid, kQuantThreads, 0, s>>>(f, x_stride, M, groups, K, row_shift, vec, out, scales);
-  }
+  auto launch = [&](auto element) {
+    using T = decltype(element);
+    auto kernel = four ? (vec ? quantize_blocks_kernel<T, ACT, 4, true> : quantize_blocks_kernel<T, ACT, 4, false>)
+                       : (vec ? quantize_blocks_kernel<T, ACT, 1, true> : quantize_blocks_kernel<T, ACT, 1, false>);
+    kernel<<<grid, kQuantThreads, 0, s>>>((const T*)x, x_stride, M, groups, K, row_shift, out, scales);
+  };
+  if (dtype == SB_BF16)
+    launch(__nv_bfloat16{});
+  else
+    launch(float{});
   SB_CHECK_LAUNCH(what);
   return SB_OK;
 }
@@ -488,9 +522,9 @@ extern "C" int sb_fp8_add_rms_norm_quantize(const void* x, int64_t x_stride, con
   p.vec = C % 4 == 0 && x_stride % 4 == 0 && (uintptr_t)x % row_bytes == 0 && (uintptr_t)out % 4 == 0 &&
           (residual == nullptr || (residual_stride % 4 == 0 && (uintptr_t)residual % row_bytes == 0 &&
                                    (uintptr_t)summed % row_bytes == 0));
-  p.vec_params = C % 4 == 0 && (gate == nullptr || (aligned16(gate) && gate_stride % 4 == 0)) &&
-                 (weight == nullptr || (aligned16(weight) && weight_stride % 4 == 0)) &&
-                 (shift == nullptr || (aligned16(shift) && shift_stride % 4 == 0));
+  p.vec = p.vec && (gate == nullptr || (aligned16(gate) && gate_stride % 4 == 0)) &&
+          (weight == nullptr || (aligned16(weight) && weight_stride % 4 == 0)) &&
+          (shift == nullptr || (aligned16(shift) && shift_stride % 4 == 0));
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == SB_BF16)
     dispatch_norm<__nv_bfloat16>(p, blocks != 0, s);
