@@ -235,15 +235,16 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = W == 1 ? 0 : warp;
   const int c0 = part * kGroup + lane * 4;  // + j * W * kGroup
-  const int64_t step = W == 1 ? (int64_t)gridDim.x * 8 : gridDim.x;
-  int64_t row = W == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
+  // Row numbers and the few steps past the last one fit 32 bits (M < 2^31).
+  const uint32_t M = (uint32_t)p.M, step = W == 1 ? gridDim.x * 8 : gridDim.x;
+  uint32_t row = W == 1 ? blockIdx.x * 8 + warp : blockIdx.x;
   const T* x = static_cast<const T*>(p.x);
   const T* res = static_cast<const T*>(p.residual);
   Raw4<T> xr[R][V], rr[R][V];
-  auto fetch = [&](int64_t at) {
+  auto fetch = [&](uint32_t at) {
 #pragma unroll
     for (int r = 0; r < R; ++r, at += step) {
-      if (at >= p.M) break;
+      if (at >= M) break;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         xr[r][j].load(x + at * p.x_stride, c0 + j * W * kGroup, p.C, VEC);
@@ -256,11 +257,18 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
     for (int i = 0; i < 4; ++i) v[i] = fill;
     if (base != nullptr) load_cols(base + at, c0 + j * W * kGroup, p.C, VEC, v);
   };
-  auto sample_of = [&](int64_t at) -> int64_t {
-    return p.rows_per_sample == p.M ? 0 : (uint32_t)at / (uint32_t)p.rows_per_sample;
+  // The rows only go forward, so a sample is looked up (a division) only past the last one's end.
+  const uint32_t per_sample = (uint32_t)p.rows_per_sample;
+  uint32_t current = 0, current_end = per_sample;
+  auto sample_of = [&](uint32_t at) {
+    if (at >= current_end) {
+      current = at / per_sample;
+      current_end = (current + 1) * per_sample;
+    }
+    return current;
   };
   float weight[KEEP ? V : 1][4], shift[KEEP ? V : 1][4];
-  int64_t kept = -1;  // the sample of weight and shift
+  uint32_t kept = ~0u;  // the sample of weight and shift
 
 #pragma unroll
   for (int r = 0; r < R; ++r)  // rows past the end are computed on zeros and not stored
@@ -269,20 +277,22 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
       xr[r][j] = Raw4<T>{};
       rr[r][j] = Raw4<T>{};
     }
-  if (row < p.M) fetch(row);
-  for (int parity = 0; row < p.M; row += R * step, parity ^= 1) {
+  if (row < M) fetch(row);
+  for (int parity = 0; row < M; row += R * step, parity ^= 1) {
     float v[R][V][4], ss[R], rstd[R], amax[R];
+    uint32_t sample[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t at = row + r * step;
-      const float* gate = p.gate == nullptr ? nullptr : p.gate + sample_of(at) * p.gate_stride;
+      const uint32_t at = row + r * step;
+      sample[r] = at < M ? sample_of(at) : 0;
+      const float* gate = p.gate == nullptr ? nullptr : p.gate + sample[r] * p.gate_stride;
       ss[r] = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         xr[r][j].get(v[r][j]);
         if (res != nullptr) {
           float s[4], g[4];
-          params(at < p.M ? gate : nullptr, 0, j, 1.f, g);
+          params(gate, 0, j, 1.f, g);
           rr[r][j].get(s);
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[r][j][i] = fmaf(g[i], v[r][j][i], s[i]);
@@ -295,10 +305,10 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
     if (res != nullptr) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (row + r * step < p.M) {
+        if (row + r * step < M) {
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            store_cols(static_cast<T*>(p.summed) + (row + r * step) * p.C, c0 + j * W * kGroup, p.C, VEC, v[r][j]);
+            store_cols(static_cast<T*>(p.summed) + (int64_t)(row + r * step) * p.C, c0 + j * W * kGroup, p.C, VEC, v[r][j]);
         }
     }
 #pragma unroll
@@ -323,24 +333,23 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t at = row + r * step;
-      if (at >= p.M) break;
-      const int64_t sample = sample_of(at);
-      if (KEEP && sample != kept) {
+      if (at >= M) break;
+      if (KEEP && sample[r] != kept) {
 #pragma unroll
         for (int j = 0; j < (KEEP ? V : 1); ++j) {
-          params(p.weight, sample * p.weight_stride, j, 1.f, weight[j]);
-          params(p.shift, sample * p.shift_stride, j, 0.f, shift[j]);
+          params(p.weight, sample[r] * p.weight_stride, j, 1.f, weight[j]);
+          params(p.shift, sample[r] * p.shift_stride, j, 0.f, shift[j]);
         }
       }
-      kept = sample;
+      kept = sample[r];
       uint8_t* out = p.out + at * p.C;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int kb = j * W + part;
         float w[4], b[4];
         if (!KEEP) {
-          params(p.weight, sample * p.weight_stride, j, 1.f, w);
-          params(p.shift, sample * p.shift_stride, j, 0.f, b);
+          params(p.weight, sample[r] * p.weight_stride, j, 1.f, w);
+          params(p.shift, sample[r] * p.shift_stride, j, 0.f, b);
         }
         // Columns past the end hold 0 * rstd (and a shift of 0), which adds nothing to the
         // maximum: rstd is NaN only where the row's values are too.
@@ -367,7 +376,7 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int64_t at = row + r * step;
-        if (at >= p.M) break;
+        if (at >= M) break;
         if (W > 1) {
           amax[r] = red[parity][1][r][0];
 #pragma unroll

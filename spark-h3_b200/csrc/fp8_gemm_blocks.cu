@@ -141,34 +141,57 @@ __device__ __forceinline__ void tile_coords(int64_t t, int m_tiles, int n_tiles,
   nt = within / gm;
 }
 
-__device__ __forceinline__ void load16(const __nv_bfloat16* p, float* v) { load8_plain(p, v); }
-__device__ __forceinline__ void load16(const float* p, float* v) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+// 16 bytes of a row of T as fp32.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& raw, float* v) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (sizeof(T) == 2) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      v[i] = __uint_as_float(w[i]);
+    }
+  }
 }
 
-// Bias, gate and residual of the 16 bytes of output columns from column n of row m applied to f.
-// The residual may be the output: its loads are plain and precede the row's store.
-template <typename T>
-__device__ __forceinline__ void finish_columns(const BlockGemmParams& p, int64_t m, bool row_ok, int n, float* f) {
-  constexpr int kVec = 16 / (int)sizeof(T);
-  if (p.bias != nullptr) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      if (n + i < p.N) f[i] += __ldg(p.bias + n + i);
-  }
-  if (p.residual != nullptr && row_ok) {
-    const T* res = static_cast<const T*>(p.residual) + m * p.N + n;
-    float r[kVec];
-    if (p.tma_out && n < p.N) {  // whole 16-byte vectors
-      load16(res, r);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) r[i] = n + i < p.N ? Elem<T>::to_f(res[i]) : 0.f;
+// A warp's 32 rows x 64 bytes between shared memory (16-byte chunk q of row r at q ^ ((r >> 1) & 3))
+// and rows m0 .. of a matrix with N columns, from column nc on; rows from M and columns from N on
+// are left out.  For matrices whose rows are no whole 16-byte vectors: four bytes per lane, two
+// rows at a time, where rows start on four bytes, else two.
+template <typename T, bool STORE>
+__device__ __forceinline__ void copy_rows(uint32_t stage, T* matrix, int64_t m0, int64_t M, int nc, int N, int lane) {
+  const int rows = (int)min((int64_t)32, M - m0);
+  if (sizeof(T) == 4 || N % 2 == 0) {
+    const int u = lane & 15, col = nc + u * (4 / (int)sizeof(T));
+    if (col >= N) return;
+    T* at = matrix + (m0 + (lane >> 4)) * N + col;
+    for (int r = lane >> 4; r < rows; r += 2, at += 2 * (int64_t)N) {
+      const uint32_t s = stage + (uint32_t)(r * 64 + (((u >> 2) ^ ((r >> 1) & 3)) * 16) + (u & 3) * 4);
+      uint32_t v;
+      if (STORE) {
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(s) : "memory");
+        *reinterpret_cast<uint32_t*>(at) = v;
+      } else {
+        v = *reinterpret_cast<const uint32_t*>(at);
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(s), "r"(v) : "memory");
+      }
     }
-#pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      if (n + i < p.N) f[i] = fmaf(p.gate != nullptr ? __ldg(p.gate + n + i) : 1.f, f[i], r[i]);
+  } else {
+    if (nc + lane >= N) return;
+    T* at = matrix + m0 * N + nc + lane;
+    for (int r = 0; r < rows; ++r, at += N) {
+      const uint32_t s = stage + (uint32_t)(r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2);
+      uint16_t v;
+      if (STORE) {
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(s) : "memory");
+        *reinterpret_cast<uint16_t*>(at) = v;
+      } else {
+        v = *reinterpret_cast<const uint16_t*>(at);
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(s), "h"(v) : "memory");
+      }
+    }
   }
 }
 
@@ -425,44 +448,66 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       if (n0 >= p.N) continue;
       // ---------------------------------------------------------- output
       const bool row_ok = m < p.M;
+      const int64_t row0 = m - lane;
+      // A lane's 16-byte chunk q of its staged row sits at q ^ ((row >> 1) & 3) (64-byte swizzle).
+      const uint32_t my_stage = stage + (uint32_t)(lane * 64), swizzle = (uint32_t)((lane >> 1) & 3);
 #pragma unroll
       for (int g = 0; g < 128 / kOutCols; ++g) {
         const int nc = n0 + g * kOutCols;
-        if (p.tma_out) {
-          if (lane == 0) bulk_wait_group_read<0>();
+        if (p.tma_out && lane == 0) bulk_wait_group_read<0>();
+        __syncwarp();  // the stage is free
+        if (!p.tma_out && p.residual != nullptr) {
+          copy_rows<T, false>(stage, static_cast<T*>(const_cast<void*>(p.residual)), row0, p.M, nc, p.N, lane);
           __syncwarp();
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {  // 16 bytes of the row at a time
+          const int n = nc + q * kVec;
+          const uint32_t chunk = my_stage + (((uint32_t)q ^ swizzle) * 16u);
           float f[kVec];
 #pragma unroll
-          for (int i = 0; i < kVec / 2; ++i) f2_unpack(acc[(g * kOutCols + q * kVec) / 2 + i], f[2 * i], f[2 * i + 1]);
-          finish_columns<T>(p, m, row_ok, nc + q * kVec, f);
-          if (p.tma_out) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = sizeof(T) == 2 ? cvt_bf16x2(f[(2 * e) % kVec], f[(2 * e + 1) % kVec]) : __float_as_uint(f[e]);
-            // chunk q of staged row r sits at q ^ ((r >> 1) & 3) (64-byte swizzle)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                             stage + (uint32_t)(lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16))),
-                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                         : "memory");
-          } else if (row_ok) {
-            T* out = static_cast<T*>(p.out) + m * p.N + nc + q * kVec;
+          for (int i = 0; i < kVec / 2; ++i)
+            f2_unpack(acc[(g * kOutCols + q * kVec) / 2 + i], f[2 * i], f[2 * i + 1]);
+          if (p.bias != nullptr) {
 #pragma unroll
             for (int i = 0; i < kVec; ++i)
-              if (nc + q * kVec + i < p.N) out[i] = Elem<T>::from_f(f[i]);
+              if (n + i < p.N) f[i] += __ldg(p.bias + n + i);
           }
+          if (p.residual != nullptr) {
+            // The residual may be the output: its loads are plain and precede the row's store.
+            uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+            if (p.tma_out) {
+              if (row_ok && n < p.N)
+                raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + m * p.N + n);
+            } else {
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(raw.x), "=r"(raw.y), "=r"(raw.z), "=r"(raw.w)
+                           : "r"(chunk)
+                           : "memory");
+            }
+            float res[kVec];
+            unpack16<T>(raw, res);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+              if (n + i < p.N) f[i] = fmaf(p.gate != nullptr ? __ldg(p.gate + n + i) : 1.f, f[i], res[i]);
+          }
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = sizeof(T) == 2 ? cvt_bf16x2(f[(2 * e) % kVec], f[(2 * e + 1) % kVec]) : __float_as_uint(f[e]);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                       : "memory");
         }
         if (p.tma_out) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {  // rows past M and columns past N are clipped by the store
-            const int64_t row0 = (int64_t)mt * 256 + rank * 128 + quad * 32;
             if (nc < p.N && row0 < p.M) tma_store_2d(&tm_out, stage, nc, (int)row0);
             bulk_commit_group();
           }
+        } else {
+          __syncwarp();
+          copy_rows<T, true>(stage, static_cast<T*>(p.out), row0, p.M, nc, p.N, lane);
         }
       }
     }
