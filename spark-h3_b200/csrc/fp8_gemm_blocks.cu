@@ -76,7 +76,7 @@ constexpr int kPairStageBytes = 2 * kPairOpBytes;  // A half + B half per CTA
 constexpr int kPairHalfBytes = 64 * kBlockK;      // a CTA's B rows of one half of the tile
 constexpr uint32_t kPairAccCols = 128;            // columns of a half; two halves x two buffers
 constexpr int kPairOutBox = 32 * 64;           // one epilogue warp's 32 rows x 64 bytes
-constexpr int kPairOutBytes = kEpiWarps * kPairOutBox;
+constexpr int kPairOutBytes = kEpiWarps * 2 * kPairOutBox;  // two boxes per warp
 constexpr int kChunkFloats = kChunk * 2 * 128;  // [k-block][weight block of the tile][row]
 constexpr int kScaleBytes = 2 * kChunkFloats * 4;
 
@@ -167,6 +167,7 @@ __device__ __forceinline__ void copy_rows(uint32_t stage, T* matrix, int64_t m0,
     const int u = lane & 15, col = nc + u * (4 / (int)sizeof(T));
     if (col >= N) return;
     T* at = matrix + (m0 + (lane >> 4)) * N + col;
+#pragma unroll 8
     for (int r = lane >> 4; r < rows; r += 2, at += 2 * (int64_t)N) {
       const uint32_t s = stage + (uint32_t)(r * 64 + (((u >> 2) ^ ((r >> 1) & 3)) * 16) + (u & 3) * 4);
       uint32_t v;
@@ -181,6 +182,7 @@ __device__ __forceinline__ void copy_rows(uint32_t stage, T* matrix, int64_t m0,
   } else {
     if (nc + lane >= N) return;
     T* at = matrix + m0 * N + nc + lane;
+#pragma unroll 8
     for (int r = 0; r < rows; ++r, at += N) {
       const uint32_t s = stage + (uint32_t)(r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2);
       uint16_t v;
@@ -384,7 +386,7 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int quad = warp & 3, half = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t stage = smem_u32(sOut) + (uint32_t)(warp * kPairOutBox);
+    const uint32_t stages = smem_u32(sOut) + (uint32_t)(warp * 2 * kPairOutBox);
     const uint32_t acc_empty = mapa_shared(smem_u32(&C.acc_empty[half]), 0);  // + 16 bytes for buffer 1
     constexpr int kOutCols = 64 / (int)sizeof(T);  // columns of a staged 64-byte row
     constexpr int kVec = 16 / (int)sizeof(T);
@@ -450,11 +452,12 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       const bool row_ok = m < p.M;
       const int64_t row0 = m - lane;
       // A lane's 16-byte chunk q of its staged row sits at q ^ ((row >> 1) & 3) (64-byte swizzle).
-      const uint32_t my_stage = stage + (uint32_t)(lane * 64), swizzle = (uint32_t)((lane >> 1) & 3);
+      const uint32_t swizzle = (uint32_t)((lane >> 1) & 3);
 #pragma unroll
       for (int g = 0; g < 128 / kOutCols; ++g) {
         const int nc = n0 + g * kOutCols;
-        if (p.tma_out && lane == 0) bulk_wait_group_read<0>();
+        const uint32_t stage = stages + (uint32_t)((g & 1) * kPairOutBox), my_stage = stage + (uint32_t)(lane * 64);
+        if (p.tma_out && lane == 0) bulk_wait_group_read<1>();  // the store before the last one
         __syncwarp();  // the stage is free
         if (!p.tma_out && p.residual != nullptr) {
           copy_rows<T, false>(stage, static_cast<T*>(const_cast<void*>(p.residual)), row0, p.M, nc, p.N, lane);
