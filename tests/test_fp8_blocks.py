@@ -631,3 +631,99 @@ def test_attention_segments_quantise_in_row_order(cuda_device):
     got = tuple(t.view(2, M, -1).transpose(0, 1).reshape(M, -1) for t in (codes, scale))
     want = fl.quantize_blocks(rows)
     assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+
+
+# ------------------------------------------------------------------------------ GPU: far offsets, neighbours, streams
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda_device):
+    """Rows that start past 2^31 elements: the last rows of a large call are those of a small one."""
+    M, K, tail = 140_000, 16_384, 5  # 2.3e9 elements
+    assert M * K > 2 ** 31
+    x = torch.zeros(M, K, device=cuda_device, dtype=torch.bfloat16)
+    x[-tail:] = torch.randn(tail, K, device=cuda_device).to(torch.bfloat16)
+    weight = torch.randn(K, device=cuda_device)
+    for call in (fl.quantize_blocks, fl.swiglu_quantize_blocks, lambda t: fl.add_rms_norm_quantize(t, weight)[:2]):
+        got, want = call(x), call(x[-tail:])
+        for a, b in zip(got, want):
+            assert torch.equal(a[-tail:].view(torch.uint8), b.view(torch.uint8))
+        del got
+    summed = fl.add_rms_norm_quantize(x, weight, x, out=x)[2]
+    assert summed is x and bool((x[:-tail] == 0).all())
+    del x, summed
+    for N, dtype in ((16_600, torch.bfloat16), (16_601, torch.bfloat16)):  # TMA stores, row by row stores
+        a, a_scale, b, b_scale, _ = gemm_inputs(131_000, N, 16, cuda_device, 2)
+        assert a.shape[0] * N > 2 ** 31
+        out = fl.fp8_gemm_blocks(a, a_scale, b, b_scale, out_dtype=dtype)
+        assert torch.equal(out[-300:], fl.fp8_gemm_blocks(a[-300:], a_scale[-300:], b, b_scale, out_dtype=dtype))
+        del out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [256, 264, 131])
+def test_kernels_leave_the_memory_around_their_outputs(cuda_device, K):
+    M, pad = 9, 512
+    x = torch.randn(M, K, device=cuda_device)
+    nb = blocks_of(K)
+    stream = torch.cuda.current_stream(cuda_device).cuda_stream
+
+    def guarded(n, dtype):
+        buf = torch.full((n + 2 * pad,), 77, device=cuda_device, dtype=dtype)
+        return buf, buf[pad:].data_ptr()
+
+    codes, codes_ptr = guarded(M * K, torch.uint8)
+    scale, scale_ptr = guarded(M * nb, torch.float32)
+    summed, summed_ptr = guarded(M * K, torch.float32)
+    _lib.call("sb_fp8_quantize_blocks", x.data_ptr(), K, _lib.F32, M, K, codes_ptr, scale_ptr, stream)
+    _lib.call("sb_fp8_add_rms_norm_quantize", x.data_ptr(), K, x.data_ptr(), K, None, 0, None, 0, None, 0, _lib.F32, M, K,
+              M, 1e-6, 1, summed_ptr, codes_ptr, scale_ptr, stream)
+    for buf, n in ((codes, M * K), (scale, M * nb), (summed, M * K)):
+        assert bool((buf[:pad] == 77).all()) and bool((buf[pad + n:] == 77).all())
+    want = fl.add_rms_norm_quantize(x, None, x)
+    assert torch.equal(codes[pad:pad + M * K].view(M, K), want[0].view(torch.uint8))
+    assert torch.equal(summed[pad:pad + M * K].view(M, K), want[2])
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(cuda_device):
+    """Split, streamed and paired GEMMs of different shapes overlap on two streams without touching
+    each other's results (there is no shared workspace)."""
+    shapes = [(2, 4096, 4096), (40, 1024, 4096), (300, 2056, 1040), (16, 4104, 5376)]
+    cases = []
+    for i, s in enumerate(shapes):
+        args = gemm_inputs(*s, cuda_device, 20 + i)[:4]
+        cases.append((args, fl.fp8_gemm_blocks(*args)))
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(2)]
+    outs = []
+    torch.cuda.synchronize()
+    for round_ in range(12):
+        for i, stream in enumerate(streams):
+            args, want = cases[(round_ + 2 * i) % len(cases)]
+            with torch.cuda.stream(stream):
+                outs.append((fl.fp8_gemm_blocks(*args), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(got, want) for got, want in outs)
+    assert ops.read_device_status(cuda_device) == 0
+
+
+@pytest.mark.gpu
+def test_results_do_not_change_from_call_to_call(cuda_device):
+    for s in ((1, 4096, 4096), (24, 14336, 1040), (64, 512, 16384), (2600, 4096, 1040)):
+        args = gemm_inputs(*s, cuda_device, 3)[:4]
+        first = fl.fp8_gemm_blocks(*args, out_dtype=torch.float32)
+        for _ in range(5):
+            assert torch.equal(fl.fp8_gemm_blocks(*args, out_dtype=torch.float32), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(300, 1001, 272), (2600, 4099, 400), (520, 131, 1040)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gemm_odd_columns_with_residual_in_place(cuda_device, M, N, K, dtype):
+    """Rows that are no whole 16-byte vectors go through shared memory in both directions."""
+    a, a_scale, b, b_scale, g = gemm_inputs(M, N, K, cuda_device, M)
+    want, error = gemm_reference(a, a_scale, b, b_scale)
+    residual = (torch.randn(M, N, device=cuda_device, generator=g) * 10).to(dtype)
+    full = residual.double() + want
+    out = fl.fp8_gemm_blocks(a, a_scale, b, b_scale, residual=residual, out=residual)
+    assert out is residual
+    assert_gemm(out, full, error + (want.abs() + full.abs()) * 2.0 ** -23)
