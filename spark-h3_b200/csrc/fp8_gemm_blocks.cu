@@ -782,6 +782,10 @@ fp8_gemm_blocks_swap_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, 913);
     return;
   }
+  if (warp == kSwapProducer && lane == 0) {
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSwapMaxStages; ++s) {
       mbar_init(smem_u32(&C.full[s]), 1);
