@@ -536,8 +536,8 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
 // For one or two rows of A the product is the reading of B once: each thread multiplies its 16
 // bytes of a weight row with its 16 columns of the M rows, which it keeps as fp32, so weights go
 // from global memory to registers with no staging, and no TMEM, barrier or tensor map has to be
-// set up.  A CTA of 8 warps takes kRows weight rows per row group; `kWarps` warps split K (512
-// columns each at a time) and the sums meet in shared memory.
+// set up.  A CTA of 8 warps takes kRows weight rows per row group; `k_warps` warps split K (512
+// columns each at a time) and the sums meet in shared memory.  1 x 4096 x 4096: 5.9 us (swap 7.3).
 constexpr int kStreamThreads = 256;
 constexpr int kRows = 8;
 
@@ -1000,6 +1000,15 @@ int launch_pair(const uint8_t* a, const uint8_t* b, BlockGemmParams p, cudaStrea
     return rc;
   p.m_tiles = (int)((p.M + 255) / 256);
   p.n_tiles = (p.N + 255) / 256;
+  // setmaxnreg waits for registers that the launch did not bring: refuse a build with other counts.
+  static const int regs = [] {
+    cudaFuncAttributes fa{};
+    return cudaFuncGetAttributes(&fa, fp8_gemm_blocks_pair_kernel<T>) == cudaSuccess ? fa.numRegs : -1;
+  }();
+  if (regs != kLaunchRegs) {
+    set_error("sb_fp8_gemm_blocks: the kernel was built with %d registers per thread, not %d", regs, kLaunchRegs);
+    return SB_ERR_UNSUPPORTED;
+  }
   const size_t smem = (size_t)kPairStages * kPairStageBytes + kPairOutBytes + kScaleBytes + sizeof(PairControl);
   cudaError_t err =
       cudaFuncSetAttribute(fp8_gemm_blocks_pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

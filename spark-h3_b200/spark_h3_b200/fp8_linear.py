@@ -138,6 +138,19 @@ def _same_device(device: torch.device, *tensors) -> None:
             raise RuntimeError(f"all tensors must be on the same CUDA device: one is on {t.device}, not {device}")
 
 
+def _refuse_overlap(out: torch.Tensor, **inputs) -> None:
+    """An output may be an input itself, laid out alike, but not overlap one in any other way: the
+    kernels read some rows after they have written others."""
+    first, last = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for name, t in inputs.items():
+        if t is None or t.numel() == 0 or out.numel() == 0:
+            continue
+        same = t.data_ptr() == first and t.dtype == out.dtype and t.shape == out.shape and t.is_contiguous()
+        span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+        if not same and t.data_ptr() < last and first < t.data_ptr() + span * t.element_size():
+            raise ValueError(f"out overlaps {name} without being it")
+
+
 def _call_on(device: torch.device, name: str, *args) -> None:
     """The C-ABI call with `device` current, on its current stream.  These operators take a few
     microseconds on a few rows, so the host side keeps to the cheapest forms of both queries."""
@@ -220,7 +233,7 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
     Returns (codes [M, C], scales, s): scales [M, ceil(C / 128)] (`blocks`, for fp8_gemm_blocks)
     or [M, 1] (for fp8_gemm); s in x's dtype, written to `out` when given (which may be the
     residual itself: the residual stream updated in place), or None without a residual.  The
-    norm works on the unrounded fp32 sum."""
+    norm works on the unrounded fp32 sum.  Outputs carry no gradient."""
     x, M, C, x_stride = _strided_rows(x, "x")
     device, dtype = x.device, _dtype_code(x)
     r_stride = 0
@@ -236,6 +249,8 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
             out = torch.empty(M, C, device=device, dtype=x.dtype)
         elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {tuple(x.shape)} {x.dtype}")
+        else:
+            _refuse_overlap(out, x=x, residual=residual, weight=weight, gate=gate, shift=shift)
     _same_device(device, residual, weight, gate, shift, out)
     samples, gate_ptr, g_stride, weight_ptr, w_stride, shift_ptr, s_stride = 1, None, 0, None, 0, None, 0
     if gate is not None:
@@ -263,7 +278,8 @@ def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Ten
     """[M, N] = a_fp8 [M, K] . b_fp8 [N, K]^T with a_scale [M, ceil(K / 128)] (any strides) applied
     per row and 128 columns and b_scale [ceil(N / 128), ceil(K / 128)] per 128 x 128 block
     (+ bias [N]); residual + gate * (that) with a residual [M, N] of the output's dtype (gate [N],
-    1 when None).  out_dtype bf16 (the default) or fp32; `out` may be the residual itself."""
+    1 when None).  out_dtype bf16 (the default) or fp32; `out` may be the residual itself.  K must
+    be a multiple of 16.  The output carries no gradient."""
     if a_fp8.dtype != FP8_DTYPE or b_fp8.dtype != FP8_DTYPE:
         raise TypeError("fp8_gemm_blocks takes float8_e4m3fn operands")
     if a_fp8.dim() != 2 or b_fp8.dim() != 2 or a_fp8.shape[1] != b_fp8.shape[1]:
@@ -289,6 +305,10 @@ def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Ten
         out = torch.empty(M, N, device=device, dtype=out_dtype)
     elif out.shape != (M, N) or out.dtype != out_dtype or not out.is_contiguous():
         raise ValueError(f"out must be contiguous [{M}, {N}] {out_dtype}")
+    else:
+        _refuse_overlap(out, a_fp8=a_fp8, a_scale=a_scale, b_fp8=b_fp8, b_scale=b_scale, bias=bias, gate=gate)
+        if residual is not None:
+            _refuse_overlap(out, residual=residual)
     code = _dtype_code(out)
     if bias is not None:
         bias = bias.float().contiguous()
@@ -404,7 +424,7 @@ class Fp8Linear(nn.Module):
         shape = x.shape
         rows = x.reshape(-1, shape[-1])
         out = self.forward_quantized(*self.quantize(rows), out_dtype=rows.dtype)
-        return out.reshape(*shape[:-1], -1)
+        return out.reshape(*shape[:-1], self.out_features)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
@@ -447,7 +467,7 @@ def forward_qkv_shared(attn, hidden_states):
     rows = hidden_states.reshape(-1, hidden_states.shape[-1])
     x_fp8, x_scale = attn.to_q.quantize(rows)
     return tuple(p.forward_quantized(x_fp8, x_scale, out_dtype=hidden_states.dtype)
-                 .reshape(*hidden_states.shape[:-1], -1) for p in projections)
+                 .reshape(*hidden_states.shape[:-1], p.out_features) for p in projections)
 
 
 class Fp8SwiGLUFeedForward(nn.Module):
@@ -467,7 +487,7 @@ class Fp8SwiGLUFeedForward(nn.Module):
         shape = hidden_states.shape
         h = self.proj(hidden_states.reshape(-1, shape[-1]))
         out = self.down.forward_quantized(*self.down.swiglu_quantize(h), out_dtype=h.dtype)
-        return out.reshape(*shape[:-1], -1)
+        return out.reshape(*shape[:-1], self.down.out_features)
 
 
 class Fp8AttnProcessor:
@@ -481,7 +501,10 @@ class Fp8AttnProcessor:
     def __call__(self, attn, hidden_states, rotary_emb=None, attention_mask=None):
         from .processor import apply_rotary_emb
 
-        query, key, value = forward_qkv_shared(attn, hidden_states)
+        projected = forward_qkv_shared(attn, hidden_states)
+        if projected is None:  # projections replaced since, or of different granularity
+            projected = (attn.to_q(hidden_states), attn.to_k(hidden_states), attn.to_v(hidden_states))
+        query, key, value = projected
         query = attn.norm_q(query.unflatten(-1, (attn.heads, -1)))
         key = attn.norm_k(key.unflatten(-1, (attn.heads, -1)))
         value = value.unflatten(-1, (attn.heads, -1))
@@ -515,7 +538,8 @@ def convert_linear_to_fp8(model, min_width=MIN_WIDTH, skip_end_blocks=SKIP_END_B
     model.transformer_blocks for Fp8Linear, in place, and fuse each converted block's SwiGLU
     FeedForward (fp8_linear.py:398-427).  `skip_end_blocks` keeps the first and last N blocks
     in bf16.  `scales`: "channel" (per token x per output channel, Fp8Linear) or "block" (per
-    128 columns x per 128 x 128 block, Fp8BlockLinear).  Returns how many Linears were swapped."""
+    128 columns x per 128 x 128 block, Fp8BlockLinear; Linears whose in_features is no multiple of
+    16 stay as they are).  Returns how many Linears were swapped."""
     if scales not in ("channel", "block"):
         raise ValueError(f'scales must be "channel" or "block", got {scales!r}')
     kind = Fp8Linear if scales == "channel" else Fp8BlockLinear
@@ -531,6 +555,8 @@ def convert_linear_to_fp8(model, min_width=MIN_WIDTH, skip_end_blocks=SKIP_END_B
                 if not isinstance(child, nn.Linear):
                     continue
                 if child.in_features < min_width or child.out_features < min_width:
+                    continue
+                if kind is Fp8BlockLinear and child.in_features % 16:
                     continue
                 setattr(parent, name, kind(child).to(child.weight.device))
                 swapped += 1

@@ -80,7 +80,7 @@ _NORM = dict(x=_P, x_stride=256, residual=_P, residual_stride=256, gate=_P, gate
     (dict(residual_stride=0), "rows overlap", -1), (dict(rows=0), "whole number of samples", -1),
     (dict(rows=3), "whole number of samples", -1), (dict(blocks=2), "blocks must be 0 or 1", -1),
     (dict(x=_P + 1), "aligned to their elements", -1), (dict(scales=_P + 2), "aligned to their elements", -1),
-    (dict(C=16385, x_stride=20000, residual_stride=20000), "at most 16384 columns", -3)])
+    (dict(shift_stride=-1), "must not be negative", -1), (dict(C=16385, x_stride=20000, residual_stride=20000), "at most 16384 columns", -3)])
 def test_norm_rejects_bad_arguments(change, message, code):
     lib = _lib.load()
     assert lib.sb_fp8_add_rms_norm_quantize(*{**_NORM, **change}.values()) == code
@@ -727,3 +727,46 @@ def test_gemm_odd_columns_with_residual_in_place(cuda_device, M, N, K, dtype):
     out = fl.fp8_gemm_blocks(a, a_scale, b, b_scale, residual=residual, out=residual)
     assert out is residual
     assert_gemm(out, full, error + (want.abs() + full.abs()) * 2.0 ** -23)
+
+
+def test_block_scales_leave_unfit_linears():
+    """in_features that is no multiple of 16 (the GEMM's row pitch): the Linear stays."""
+    model = nn.Module()
+    model.transformer_blocks = nn.ModuleList([nn.Sequential(nn.Linear(24, 32), nn.Linear(32, 24))])
+    assert fl.convert_linear_to_fp8(model, min_width=8, scales="block") == 1
+    assert type(model.transformer_blocks[0][0]) is nn.Linear
+    assert type(model.transformer_blocks[0][1]) is fl.Fp8BlockLinear
+
+
+@pytest.mark.gpu
+def test_outputs_that_overlap_an_input_are_refused(cuda_device):
+    buf = torch.randn(9, 256, device=cuda_device).to(torch.bfloat16)
+    with pytest.raises(ValueError, match="overlaps residual"):
+        fl.add_rms_norm_quantize(torch.randn(8, 256, device=cuda_device).to(torch.bfloat16), None, buf[:8], out=buf[1:])
+    wide = torch.randn(8, 512, device=cuda_device).to(torch.bfloat16)
+    with pytest.raises(ValueError, match="overlaps x"):  # the same address, another layout
+        fl.add_rms_norm_quantize(wide[:, :256], None, buf[:8], out=wide.view(-1)[:8 * 256].view(8, 256))
+    a, a_scale, b, b_scale, _ = gemm_inputs(8, 256, 256, cuda_device, 1)
+    with pytest.raises(ValueError, match="overlaps residual"):
+        fl.fp8_gemm_blocks(a, a_scale, b, b_scale, residual=buf[:8], out=buf[1:])
+    a, a_scale, b, b_scale, _ = gemm_inputs(8, 128, 256, cuda_device, 1)
+    with pytest.raises(ValueError, match="overlaps a_fp8"):
+        fl.fp8_gemm_blocks(a, a_scale, b, b_scale, out=a.view(torch.bfloat16))  # [8, 128]
+
+
+@pytest.mark.gpu
+def test_processor_projects_one_by_one_where_granularities_differ(cuda_device):
+    from test_gpu_plugin import TinyAttention
+
+    torch.manual_seed(4)
+    attn = TinyAttention(hidden=128, heads=1).to(cuda_device, torch.bfloat16).eval()
+    x = torch.randn(1, 70, 128, device=cuda_device, dtype=torch.bfloat16)
+    processor = fl.Fp8AttnProcessor()
+    with torch.no_grad():
+        attn.to_q, attn.to_v = fl.Fp8BlockLinear(attn.to_q), fl.Fp8BlockLinear(attn.to_v)
+        mixed = processor(attn, x)
+        attn.to_k = fl.Fp8BlockLinear(attn.to_k)
+        shared = processor(attn, x)
+    assert mixed.isfinite().all() and F.cosine_similarity(mixed.flatten().float(), shared.flatten().float(), dim=0) > 0.99
+    empty = fl.Fp8BlockLinear(nn.Linear(64, 32, device=cuda_device, dtype=torch.bfloat16))
+    assert empty(x.new_empty(0, 64)).shape == (0, 32)
