@@ -5,6 +5,7 @@
 // result: each block's 128-deep partial product is finished in TMEM on its own, read back, and
 // added with its scale to an fp32 accumulator in registers.
 #include <algorithm>
+#include <atomic>
 
 #include <cuda_fp16.h>
 
@@ -1001,13 +1002,16 @@ int launch_pair(const uint8_t* a, const uint8_t* b, BlockGemmParams p, cudaStrea
   p.m_tiles = (int)((p.M + 255) / 256);
   p.n_tiles = (p.N + 255) / 256;
   // setmaxnreg waits for registers that the launch did not bring: refuse a build with other counts.
-  static const int regs = [] {
+  static std::atomic<bool> fits{false};
+  if (!fits.load(std::memory_order_relaxed)) {
     cudaFuncAttributes fa{};
-    return cudaFuncGetAttributes(&fa, fp8_gemm_blocks_pair_kernel<T>) == cudaSuccess ? fa.numRegs : -1;
-  }();
-  if (regs != kLaunchRegs) {
-    set_error("sb_fp8_gemm_blocks: the kernel was built with %d registers per thread, not %d", regs, kLaunchRegs);
-    return SB_ERR_UNSUPPORTED;
+    cudaError_t e = cudaFuncGetAttributes(&fa, fp8_gemm_blocks_pair_kernel<T>);
+    if (e != cudaSuccess) return cuda_error(e, "sb_fp8_gemm_blocks: kernel attributes");
+    if (fa.numRegs != kLaunchRegs) {
+      set_error("sb_fp8_gemm_blocks: the kernel was built with %d registers per thread, not %d", fa.numRegs, kLaunchRegs);
+      return SB_ERR_UNSUPPORTED;
+    }
+    fits.store(true, std::memory_order_relaxed);
   }
   const size_t smem = (size_t)kPairStages * kPairStageBytes + kPairOutBytes + kScaleBytes + sizeof(PairControl);
   cudaError_t err =
