@@ -429,9 +429,8 @@ int sb_fp8_add_rms_norm_quantize(const void* x, int64_t x_stride, const void* re
  * reference, whose GEMM takes per-row or per-tensor scales, fp8_linear.py:147-156):
  *   out[m, n] = sum_b a_scale[m, b] * b_scale[n / 128, b] * sum_{k in block b} a[m, k] * b[n, k]
  *               + bias[n],   and residual[m, n] + gate[n] * (that) with a residual.
- * Blocks are summed in order of b in fp32 (where a few rows leave the GPU idle, K is split into
- * up to 8 runs of blocks whose sums are added in order: a fixed choice by M, N, K and the number
- * of SMs).
+ * Sums are fp32, in an order that M, N, K and the number of SMs fix (K may be split into up to 8
+ * runs of blocks): the same call gives the same bits, a row of another batch size may not.
  * a: [M, K] e4m3; a_scale[m * a_row_stride + b * a_block_stride] fp32; b: [N, K] e4m3 (the
  * weight, K-major); b_scale: [ceil(N / 128), ceil(K / 128)] fp32; bias, gate: [N] fp32 or NULL;
  * residual: [M, N] of the output's type or NULL (it may be the output); a NULL gate is 1; out: [M, N]

@@ -26,7 +26,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from .ops import _dtype_code, _ptr, _require_cuda, _stream
+from .ops import _dtype_code, _require_cuda, _stream
 
 FP8_DTYPE = torch.float8_e4m3fn
 FP8_MAX = 448.0
@@ -131,11 +131,10 @@ def _strided_rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, i
     return x, M, C, stride if M > 1 else C
 
 
-def _same_device(device: torch.device, *tensors) -> None:
-    index = device.index
+def _same_device(index: int, *tensors) -> None:
     for t in tensors:
         if t is not None and t.get_device() != index:
-            raise RuntimeError(f"all tensors must be on the same CUDA device: one is on {t.device}, not {device}")
+            raise RuntimeError(f"all tensors must be on the same CUDA device: one is on {t.device}, not cuda:{index}")
 
 
 def _refuse_overlap(out: torch.Tensor, **inputs) -> None:
@@ -151,17 +150,15 @@ def _refuse_overlap(out: torch.Tensor, **inputs) -> None:
             raise ValueError(f"out overlaps {name} without being it")
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """The C-ABI call with `device` current, on its current stream.  These operators take a few
-    microseconds on a few rows, so the host side keeps to the cheapest forms of both queries."""
-    index = device.index
+def _call_on(index: int, name: str, *args) -> None:
+    """The C-ABI call with CUDA device `index` current, on its current stream.  These operators take
+    a few microseconds on a few rows, so the host side keeps to the cheapest forms of its queries."""
     fn = _lib.bound(name)
-    stream = torch._C._cuda_getCurrentRawStream(index)
     if torch._C._cuda_getDevice() == index:
-        status = fn(*args, stream)
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            status = fn(*args, stream)
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status < 0:
         _lib.check(status, name)
 
@@ -177,7 +174,7 @@ def _quantize_blocks(entry: str, x: torch.Tensor, halves: int):
     y = torch.empty(M, K, device=device, dtype=FP8_DTYPE)
     scale = torch.empty(M, -(-K // BLOCK), device=device, dtype=torch.float32)
     if M > 0:
-        _call_on(device, entry, x.data_ptr(), stride, dtype, M, K, y.data_ptr(), scale.data_ptr())
+        _call_on(device.index, entry, x.data_ptr(), stride, dtype, M, K, y.data_ptr(), scale.data_ptr())
     return y, scale
 
 
@@ -236,7 +233,7 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
     norm works on the unrounded fp32 sum.  Outputs carry no gradient."""
     x, M, C, x_stride = _strided_rows(x, "x")
     device, dtype = x.device, _dtype_code(x)
-    r_stride = 0
+    r_stride, residual_ptr, out_ptr = 0, None, None
     if residual is None:
         if gate is not None or out is not None:
             raise ValueError("gate and out belong to the residual's addition: pass a residual")
@@ -251,7 +248,8 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
             raise ValueError(f"out must be contiguous {tuple(x.shape)} {x.dtype}")
         else:
             _refuse_overlap(out, x=x, residual=residual, weight=weight, gate=gate, shift=shift)
-    _same_device(device, residual, weight, gate, shift, out)
+        residual_ptr, out_ptr = residual.data_ptr(), out.data_ptr()
+    _same_device(device.index, residual, weight, gate, shift, out)
     samples, gate_ptr, g_stride, weight_ptr, w_stride, shift_ptr, s_stride = 1, None, 0, None, 0, None, 0
     if gate is not None:
         gate, g_stride, samples = _sample_vector(gate, "gate", M, C, samples)
@@ -265,9 +263,9 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
     y = torch.empty(M, C, device=device, dtype=FP8_DTYPE)
     scale = torch.empty(M, _blocks(C) if blocks else 1, device=device, dtype=torch.float32)
     if M > 0:
-        _call_on(device, "sb_fp8_add_rms_norm_quantize", x.data_ptr(), x_stride, _ptr(residual), r_stride, gate_ptr,
+        _call_on(device.index, "sb_fp8_add_rms_norm_quantize", x.data_ptr(), x_stride, residual_ptr, r_stride, gate_ptr,
                  g_stride, weight_ptr, w_stride, shift_ptr, s_stride, dtype, M, C, M // samples, eps, 1 if blocks else 0,
-                 _ptr(out), y.data_ptr(), scale.data_ptr())
+                 out_ptr, y.data_ptr(), scale.data_ptr())
     return y, scale, out
 
 
@@ -286,49 +284,52 @@ def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Ten
         raise ValueError(f"A [M, K] and B [N, K] must share K: {tuple(a_fp8.shape)} vs {tuple(b_fp8.shape)}")
     if not a_fp8.is_cuda:
         raise RuntimeError("spark_h3_b200 kernels require CUDA tensors; there is no CPU path")
-    device = a_fp8.device
-    _same_device(device, a_scale, b_fp8, b_scale, bias, residual, gate, out)
-    a_fp8, b_fp8, b_scale = a_fp8.contiguous(), b_fp8.contiguous(), b_scale.contiguous()
+    index = a_fp8.get_device()
+    _same_device(index, a_scale, b_fp8, b_scale)
     (M, K), N = a_fp8.shape, b_fp8.shape[0]
-    kb = -(-K // BLOCK)
     if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
         raise TypeError(f"{'b' if a_scale.dtype == torch.float32 else 'a'}_scale must be float32")
+    kb = -(-K // BLOCK)
     if a_scale.shape != (M, kb):
         raise ValueError(f"a_scale must be [{M}, {kb}], got {tuple(a_scale.shape)}")
     if b_scale.shape != (-(-N // BLOCK), kb):
         raise ValueError(f"b_scale must be [{_blocks(N)}, {kb}], got {tuple(b_scale.shape)}")
-    if out is not None:
-        out_dtype = out_dtype or out.dtype
-    elif out_dtype is None:
-        out_dtype = torch.bfloat16
+    a_fp8, b_fp8, b_scale = a_fp8.contiguous(), b_fp8.contiguous(), b_scale.contiguous()
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if out is None else out.dtype
     if out is None:
-        out = torch.empty(M, N, device=device, dtype=out_dtype)
-    elif out.shape != (M, N) or out.dtype != out_dtype or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous [{M}, {N}] {out_dtype}")
+        out = torch.empty(M, N, device=a_fp8.device, dtype=out_dtype)
     else:
-        _refuse_overlap(out, a_fp8=a_fp8, a_scale=a_scale, b_fp8=b_fp8, b_scale=b_scale, bias=bias, gate=gate)
-        if residual is not None:
-            _refuse_overlap(out, residual=residual)
+        if out.shape != (M, N) or out.dtype != out_dtype or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous [{M}, {N}] {out_dtype}")
+        _same_device(index, out)
+        _refuse_overlap(out, a_fp8=a_fp8, a_scale=a_scale, b_fp8=b_fp8, b_scale=b_scale, bias=bias, gate=gate,
+                        residual=residual)
     code = _dtype_code(out)
+    bias_ptr = residual_ptr = gate_ptr = None
     if bias is not None:
+        _same_device(index, bias)
         bias = bias.float().contiguous()
         if bias.numel() != N:
             raise ValueError(f"bias needs {N} values, got {bias.numel()}")
+        bias_ptr = bias.data_ptr()
     if residual is not None:
         if residual.shape != (M, N) or residual.dtype != out_dtype:
             raise ValueError(f"the residual must be [{M}, {N}] {out_dtype}")
+        _same_device(index, residual, gate)
         residual = residual.contiguous()
+        residual_ptr = residual.data_ptr()
         if gate is not None:
             gate = gate.float().contiguous()
             if gate.numel() != N:
                 raise ValueError(f"gate needs {N} values, got {gate.numel()}")
+            gate_ptr = gate.data_ptr()
     elif gate is not None:
         raise ValueError("gate belongs to the residual's addition: pass a residual")
     if M > 0 and N > 0:
         row_stride, block_stride = a_scale.stride()
-        _call_on(device, "sb_fp8_gemm_blocks", a_fp8.data_ptr(), a_scale.data_ptr(), row_stride, block_stride,
-                 b_fp8.data_ptr(), b_scale.data_ptr(), M, N, K, _ptr(bias), _ptr(residual),
-                 _ptr(gate), out.data_ptr(), code)
+        _call_on(index, "sb_fp8_gemm_blocks", a_fp8.data_ptr(), a_scale.data_ptr(), row_stride, block_stride,
+                 b_fp8.data_ptr(), b_scale.data_ptr(), M, N, K, bias_ptr, residual_ptr, gate_ptr, out.data_ptr(), code)
     return out
 
 
