@@ -1065,32 +1065,39 @@ int launch_swap(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, Sw
   return SB_OK;
 }
 
-// Which kernel, and its shape.  The estimates are fits (in us, within about 20 %) of times measured
-// on one B200 with K of 4096 to 16384 and weights that come from HBM:
-//   pair: 6 + 0.45 per k-block and wave of tiles (one 256 x 256 tile per CTA pair);
-//   swap: 6 + 0.55 (up to 32 rows: 0.30) per k-block of a CTA with one CTA per SM, 0.70 (0.55) with
-//         two, + 3 where a cluster adds up its splits.
-// Both sides at M x N x K: 64 x 4096 x 4096 swap 11.5, pair 20.1; 1000 x 392 x 4112 15.0, 22.5;
-// 64 x 28672 x 5376 36.5, 47; 256 x 4096 x 4096 22.5, 20.1; 128 x 14336 x 5376 34.9, 29.6.
+// Which kernel, and its shape.  The estimates are fits (in us, most within 20 %) of times measured on
+// one B200, launch included, over 3 to 5208 rows, 76 to 28672 columns and K of 192 to 16384:
+//   pair: 7.5 + 0.43 per k-block and wave of tiles (one 256 x 256 tile per CTA pair);
+//   swap: 4.5, + 2 where a cluster adds up its splits of K, + 2.5 with more than one CTA per SM, + the
+//         larger of the weights' bytes at 5.5 TB/s and 0.55 (up to 32 rows of A: 0.20) per k-block
+//         of a CTA, 0.78 (0.35) with two CTAs per SM.
+// Both sides, swap and pair, at M x N x K: 64 x 4096 x 4096 11.5, 20.1; 85 x 143 x 1952 7.1, 13.4;
+// 1000 x 392 x 4112 15.0, 22.5; 64 x 28672 x 5376 36.0, 47; 2659 x 167 x 1536 12.1, 13.3;
+// 256 x 4096 x 4096 22.5, 20.1; 128 x 14336 x 5376 34.9, 29.6; 5000 x 256 x 2048 18.4, 13.9.
 double pair_estimate(int64_t M, int N, int k_blocks, int sms) {
-  const int64_t tiles = (M + 255) / 256 * ((N + 255) / 256), pairs = sms / 2;
-  return 6.0 + 0.45 * (double)((tiles + pairs - 1) / pairs) * k_blocks;
+  const int64_t tiles = (M + 255) / 256 * (((int64_t)N + 255) / 256), pairs = sms / 2;
+  return 7.5 + 0.43 * (double)((tiles + pairs - 1) / pairs) * k_blocks;
 }
 
 double swap_shape(int64_t M, int N, int k_blocks, int sms, SwapShape* shape) {
   SwapShape q{};
-  q.m_tiles = (int)((M + kSwapTokens - 1) / kSwapTokens);
-  q.tokens = (int)(((M + q.m_tiles - 1) / q.m_tiles + 15) / 16 * 16);
+  const int64_t m_tiles = (M + kSwapTokens - 1) / kSwapTokens;
+  const int64_t tiles = m_tiles * (((int64_t)N + 127) / 128);
+  if (tiles > 8 * (int64_t)sms && m_tiles > 1) return 1e30;  // never the better one, and a grid of any size
+  q.m_tiles = (int)m_tiles;
+  q.tokens = (int)(((M + m_tiles - 1) / m_tiles + 15) / 16 * 16);
   const bool narrow = q.tokens <= 32;
-  const int64_t tiles = (int64_t)q.m_tiles * ((N + 127) / 128);
+  const double weights = (double)N * k_blocks * kBlockK / 5.5e6;
   double best = 0;
-  // Splits of K by 1, 2, 4 or 8, each of at least eight k-blocks; two CTAs per SM are resident.
-  for (int splits = 1; splits <= 8 && (splits == 1 || k_blocks >= 8 * splits); splits *= 2) {
+  // Splits of K by 1, 2, 4 or 8, each of at least two k-blocks, as long as all CTAs are resident (two
+  // per SM): 64 x 28672 x 5376 split by 8 takes 76 us.
+  for (int splits = 1; splits <= 8; splits *= 2) {
     const int64_t ctas = tiles * splits;
+    if (splits > 1 && (k_blocks < 2 * splits || ctas > 2 * sms)) break;
     const int64_t waves = (ctas + 2 * sms - 1) / (2 * sms);
     const bool one = ctas <= sms;
-    const double t = 6.0 + (splits > 1 ? 3.0 : 0.0) +
-                     (one ? (narrow ? 0.30 : 0.55) : (narrow ? 0.55 : 0.70)) * (double)waves * k_blocks / splits;
+    const double loop = (one ? (narrow ? 0.20 : 0.55) : (narrow ? 0.35 : 0.78)) * (double)waves * k_blocks / splits;
+    const double t = 4.5 + (splits > 1 ? 2.0 : 0.0) + (one ? 0.0 : 2.5) + std::max(loop, weights);
     if (splits == 1 || t < best) {
       best = t;
       q.splits = splits;
@@ -1114,8 +1121,7 @@ int dispatch(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, cudaS
   const int sms = sm_count();
   SwapShape q{};
   const double pair = pair_estimate(p.M, p.N, p.k_blocks, sms);
-  // An estimate of swap beyond 2048 rows would never win, and its grid would outgrow 32 bits.
-  if (p.M <= 2048 && swap_shape(p.M, p.N, p.k_blocks, sms, &q) < pair) {
+  if (swap_shape(p.M, p.N, p.k_blocks, sms, &q) < pair) {
     if (q.tokens <= 16) return launch_swap<T, 16>(a, b, p, q, s);
     if (q.tokens <= 32) return launch_swap<T, 32>(a, b, p, q, s);
     return launch_swap<T, 64>(a, b, p, q, s);
