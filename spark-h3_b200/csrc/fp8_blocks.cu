@@ -49,57 +49,88 @@ __device__ __forceinline__ float reciprocal(float x) {
 }
 __device__ __forceinline__ float group_scale(float absmax) { return max_nan(absmax * kInv448, 1e-12f); }
 
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float* v) {
-  const uint2 raw = *reinterpret_cast<const uint2*>(p);
-  v[0] = __uint_as_float(raw.x << 16);
-  v[1] = __uint_as_float(raw.x & 0xffff0000u);
-  v[2] = __uint_as_float(raw.y << 16);
-  v[3] = __uint_as_float(raw.y & 0xffff0000u);
+// N (1, 2 or 4) consecutive elements in one access.
+template <int N>
+__device__ __forceinline__ void load_n(const __nv_bfloat16* p, float* v) {
+  if (N == 1) {
+    v[0] = __bfloat162float(*p);
+  } else {
+    uint32_t w[N / 2 > 0 ? N / 2 : 1];
+    if (N == 4) {
+      const uint2 raw = *reinterpret_cast<const uint2*>(p);
+      w[0] = raw.x;
+      w[N / 2 - 1] = raw.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
 }
-__device__ __forceinline__ void load4(const float* p, float* v) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+template <int N>
+__device__ __forceinline__ void load_n(const float* p, float* v) {
+  if (N == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[N - 2] = a.z; v[N - 1] = a.w;
+  } else if (N == 2) {
+    const float2 a = *reinterpret_cast<const float2*>(p);
+    v[0] = a.x; v[N - 1] = a.y;
+  } else {
+    v[0] = *p;
+  }
 }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(sm100::cvt_bf16x2(v[0], v[1]), sm100::cvt_bf16x2(v[2], v[3]));
+template <int N>
+__device__ __forceinline__ void store_n(__nv_bfloat16* p, const float* v) {
+  if (N == 4)
+    *reinterpret_cast<uint2*>(p) = make_uint2(sm100::cvt_bf16x2(v[0], v[N > 1 ? 1 : 0]),
+                                              sm100::cvt_bf16x2(v[N - 2 > 0 ? N - 2 : 0], v[N - 1]));
+  else if (N == 2)
+    *reinterpret_cast<uint32_t*>(p) = sm100::cvt_bf16x2(v[0], v[N - 1]);
+  else
+    *p = __float2bfloat16_rn(v[0]);
 }
-__device__ __forceinline__ void store4(float* p, const float* v) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+template <int N>
+__device__ __forceinline__ void store_n(float* p, const float* v) {
+  if (N == 4)
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[N > 1 ? 1 : 0], v[N - 2 > 0 ? N - 2 : 0], v[N - 1]);
+  else if (N == 2)
+    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[N - 1]);
+  else
+    *p = v[0];
 }
 
-// 4 values from column c of a row with `cols` columns; columns past the end read as `fill`.  `vec`:
-// the row's groups of four are aligned to their size (its columns are then a multiple of 4).
-template <typename T>
-__device__ __forceinline__ void load_cols(const T* row, int c, int cols, bool vec, float* v, float fill = 0.f) {
+// A lane's four values from column c of a row with `cols` columns, N at a time (cols is then a
+// multiple of N and the row's elements are aligned to N); columns past the end read as 0.
+template <int N, typename T>
+__device__ __forceinline__ void load_cols(const T* row, int c, int cols, float* v) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = fill;
-  if (vec) {
-    if (c < cols) load4(row + c, v);
-  } else {
+  for (int i = 0; i < 4; ++i) v[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < cols) v[i] = Elem<T>::to_f(row[c + i]);
-  }
+  for (int i = 0; i < 4; i += N)
+    if (c + i < cols) load_n<N>(row + c + i, v + i);
 }
-template <typename T>
-__device__ __forceinline__ void store_cols(T* row, int c, int cols, bool vec, const float* v) {
-  if (vec) {
-    if (c < cols) store4(row + c, v);
-  } else {
+template <int N, typename T>
+__device__ __forceinline__ void store_cols(T* row, int c, int cols, const float* v) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < cols) row[c + i] = Elem<T>::from_f(v[i]);
-  }
+  for (int i = 0; i < 4; i += N)
+    if (c + i < cols) store_n<N>(row + c + i, v + i);
 }
 // Codes of 4 values; cvt.satfinite clamps to +-448 and keeps NaN.
-__device__ __forceinline__ void store_codes(uint8_t* row, int c, int cols, bool vec, const float* v, float inv) {
+template <int N>
+__device__ __forceinline__ void store_codes(uint8_t* row, int c, int cols, const float* v, float inv) {
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v[1] * inv), "f"(v[0] * inv));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v[3] * inv), "f"(v[2] * inv));
-  const uint32_t codes = (uint32_t)lo | (uint32_t)hi << 16;
-  if (vec) {
-    if (c < cols) *reinterpret_cast<uint32_t*>(row + c) = codes;
+  if (N == 4) {
+    if (c < cols) *reinterpret_cast<uint32_t*>(row + c) = (uint32_t)lo | (uint32_t)hi << 16;
+  } else if (N == 2) {
+    if (c < cols) *reinterpret_cast<uint16_t*>(row + c) = lo;
+    if (c + 2 < cols) *reinterpret_cast<uint16_t*>(row + c + 2) = hi;
   } else {
+    const uint32_t codes = (uint32_t)lo | (uint32_t)hi << 16;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (c + i < cols) row[c + i] = (uint8_t)(codes >> (8 * i));
@@ -132,7 +163,7 @@ __device__ __forceinline__ float gelu(float x) {
 // blockIdx.y counts further 8 * U groups.
 constexpr int kQuantThreads = 256;
 
-template <typename T, int ACT, int U, bool VEC>
+template <typename T, int ACT, int U, int N>
 __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const T* __restrict__ x, int64_t x_stride,
                                                                         int64_t M, int groups, int K, int row_shift,
                                                                         uint8_t* __restrict__ out,
@@ -147,8 +178,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const T*
   float v[U][4], w[ACT == kSwiglu ? U : 1][4];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    load_cols(xr, c0 + u * kGroup, K, VEC, v[u]);
-    if (ACT == kSwiglu) load_cols(xr + K, c0 + u * kGroup, K, VEC, w[u]);
+    load_cols<N>(xr, c0 + u * kGroup, K, v[u]);
+    if (ACT == kSwiglu) load_cols<N>(xr + K, c0 + u * kGroup, K, w[u]);
   }
   float mine = 0.f;
 #pragma unroll
@@ -162,7 +193,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const T*
     }
     const float scale = group_scale(warp_absmax(absmax4(v[u])));
     if (lane == u) mine = scale;
-    store_codes(yr, c0 + u * kGroup, K, VEC, v[u], reciprocal(scale));
+    store_codes<N>(yr, c0 + u * kGroup, K, v[u], reciprocal(scale));
   }
   if (lane < U && g0 + lane < groups) scales[row * groups + g0 + lane] = mine;
 }
@@ -180,7 +211,6 @@ struct NormParams {
   int64_t gate_stride, weight_stride, shift_stride;  // floats between samples
   int64_t M, rows_per_sample;
   int C, groups;
-  int vec;  // everything is aligned for accesses of four elements
   float eps;
 };
 
@@ -188,10 +218,14 @@ struct NormParams {
 template <typename T> struct Raw4;
 template <> struct Raw4<__nv_bfloat16> {
   uint2 r;
-  __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int cols, bool vec) {
+  template <int N>
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int cols) {
     r = make_uint2(0u, 0u);
-    if (vec) {
+    if (N == 4) {
       if (c < cols) r = *reinterpret_cast<const uint2*>(row + c);
+    } else if (N == 2) {
+      if (c < cols) r.x = *reinterpret_cast<const uint32_t*>(row + c);
+      if (c + 2 < cols) r.y = *reinterpret_cast<const uint32_t*>(row + c + 2);
     } else {
       const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
       if (c + 0 < cols) r.x = h[c];
@@ -209,7 +243,8 @@ template <> struct Raw4<__nv_bfloat16> {
 };
 template <> struct Raw4<float> {
   float r[4];
-  __device__ __forceinline__ void load(const float* row, int c, int cols, bool vec) { load_cols(row, c, cols, vec, r); }
+  template <int N>
+  __device__ __forceinline__ void load(const float* row, int c, int cols) { load_cols<N>(row, c, cols, r); }
   __device__ __forceinline__ void get(float* v) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = r[i];
@@ -227,8 +262,8 @@ constexpr int norm_ctas(int W, int V) { return (V == 4 ? 512 : 768) / norm_threa
 // (unconverted) meanwhile.  The sum is rounded once, where it is stored; the norm works on the
 // unrounded fp32 sum.  Measured at 124992 x 4096 bf16 with residual, gate and shift (3.6 GB): 583 us,
 // 6.2 TB/s; 64-bit row arithmetic 615, one row at a time 659, one row per CTA without rows in flight
-// 832, access-by-access alignment checks instead of VEC 746.
-template <typename T, int W, int V, int R, bool BLOCKS, bool VEC>
+// 832, access-by-access alignment checks instead of the template's 746.
+template <typename T, int W, int V, int R, bool BLOCKS, int N>
 __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm_quantize_kernel(NormParams p) {
   constexpr bool KEEP = norm_keeps(V);
   __shared__ float red[2][2][R][W];  // [parity][sum, maximum][row][warp]
@@ -247,15 +282,18 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
       if (at >= M) break;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        xr[r][j].load(x + at * p.x_stride, c0 + j * W * kGroup, p.C, VEC);
-        if (res != nullptr) rr[r][j].load(res + at * p.residual_stride, c0 + j * W * kGroup, p.C, VEC);
+        xr[r][j].template load<N>(x + at * p.x_stride, c0 + j * W * kGroup, p.C);
+        if (res != nullptr) rr[r][j].template load<N>(res + at * p.residual_stride, c0 + j * W * kGroup, p.C);
       }
     }
   };
   auto params = [&](const float* base, int64_t at, int j, float fill, float* v) {
+    if (base != nullptr) {
+      load_cols<N>(base + at, c0 + j * W * kGroup, p.C, v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fill;
-    if (base != nullptr) load_cols(base + at, c0 + j * W * kGroup, p.C, VEC, v);
+      for (int i = 0; i < 4; ++i) v[i] = fill;
+    }
   };
   // The rows only go forward, so a sample is looked up (a division) only past the last one's end.
   const uint32_t per_sample = (uint32_t)p.rows_per_sample;
@@ -308,7 +346,7 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
         if (row + r * step < M) {
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            store_cols(static_cast<T*>(p.summed) + (int64_t)(row + r * step) * p.C, c0 + j * W * kGroup, p.C, VEC, v[r][j]);
+            store_cols<N>(static_cast<T*>(p.summed) + (int64_t)(row + r * step) * p.C, c0 + j * W * kGroup, p.C, v[r][j]);
         }
     }
 #pragma unroll
@@ -360,7 +398,7 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
         if (BLOCKS) {
           const float scale = group_scale(warp_absmax(m));
           if (lane == 0 && kb < p.groups) p.scales[at * p.groups + kb] = scale;
-          store_codes(out, c0 + j * W * kGroup, p.C, VEC, v[r][j], reciprocal(scale));
+          store_codes<N>(out, c0 + j * W * kGroup, p.C, v[r][j], reciprocal(scale));
         } else {
           amax[r] = max_nan(amax[r], m);
         }
@@ -386,7 +424,7 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
         if (part == 0 && lane == 0) p.scales[at] = scale;
         const float inv = reciprocal(scale);
 #pragma unroll
-        for (int j = 0; j < V; ++j) store_codes(p.out + at * p.C, c0 + j * W * kGroup, p.C, VEC, v[r][j], inv);
+        for (int j = 0; j < V; ++j) store_codes<N>(p.out + at * p.C, c0 + j * W * kGroup, p.C, v[r][j], inv);
       }
     }
   }
@@ -399,33 +437,36 @@ int sm_count() {
   return sms;
 }
 
-template <typename T, int W, int V>
-void launch_norm(const NormParams& p, bool blocks, cudaStream_t s) {
+template <typename T, int W, int V, int N>
+void launch_norm_n(const NormParams& p, bool blocks, cudaStream_t s) {
   // Two rows at a time where their unconverted columns take few registers.
   constexpr int kTogether = sizeof(T) == 2 && norm_keeps(V) && W > 1 ? 2 : 1;
   const int64_t ctas = W == 1 ? (p.M + 7) / 8 : p.M, resident = (int64_t)sm_count() * norm_ctas(W, V);
   const unsigned grid = (unsigned)(ctas < resident ? ctas : resident);
-  auto kernel = blocks ? (p.vec ? add_rms_norm_quantize_kernel<T, W, V, kTogether, true, true>
-                                : add_rms_norm_quantize_kernel<T, W, V, kTogether, true, false>)
-                       : (p.vec ? add_rms_norm_quantize_kernel<T, W, V, kTogether, false, true>
-                                : add_rms_norm_quantize_kernel<T, W, V, kTogether, false, false>);
-  kernel<<<grid, norm_threads(W), 0, s>>>(p);
+  if (blocks)
+    add_rms_norm_quantize_kernel<T, W, V, kTogether, true, N><<<grid, norm_threads(W), 0, s>>>(p);
+  else
+    add_rms_norm_quantize_kernel<T, W, V, kTogether, false, N><<<grid, norm_threads(W), 0, s>>>(p);
 }
 
-template <typename T>
+template <typename T, int N>
 void dispatch_norm(const NormParams& p, bool blocks, cudaStream_t s) {
-  if (p.C <= 128) return launch_norm<T, 1, 1>(p, blocks, s);
-  if (p.C <= 256) return launch_norm<T, 1, 2>(p, blocks, s);
-  if (p.C <= 512) return launch_norm<T, 1, 4>(p, blocks, s);
-  if (p.C <= 1024) return launch_norm<T, 4, 2>(p, blocks, s);
-  if (p.C <= 2048) return launch_norm<T, 8, 2>(p, blocks, s);
-  if (p.C <= 4096) return launch_norm<T, 8, 4>(p, blocks, s);
-  if (p.C <= 6144) return launch_norm<T, 12, 4>(p, blocks, s);
-  if (p.C <= 8192) return launch_norm<T, 16, 4>(p, blocks, s);
-  return launch_norm<T, 24, 6>(p, blocks, s);
+  if (p.C <= 128) return launch_norm_n<T, 1, 1, N>(p, blocks, s);
+  if (p.C <= 256) return launch_norm_n<T, 1, 2, N>(p, blocks, s);
+  if (p.C <= 512) return launch_norm_n<T, 1, 4, N>(p, blocks, s);
+  if (p.C <= 1024) return launch_norm_n<T, 4, 2, N>(p, blocks, s);
+  if (p.C <= 2048) return launch_norm_n<T, 8, 2, N>(p, blocks, s);
+  if (p.C <= 4096) return launch_norm_n<T, 8, 4, N>(p, blocks, s);
+  if (p.C <= 6144) return launch_norm_n<T, 12, 4, N>(p, blocks, s);
+  if (p.C <= 8192) return launch_norm_n<T, 16, 4, N>(p, blocks, s);
+  return launch_norm_n<T, 24, 6, N>(p, blocks, s);
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
+// Whether everything allows accesses of n elements: element counts and strides that are multiples of
+// n, pointers aligned to n elements (size bytes each).
+bool fits(int n, const void* p, int size, int64_t stride = 0) {
+  return p == nullptr || ((uintptr_t)p % (uintptr_t)(n * size) == 0 && stride % n == 0);
+}
 
 template <int ACT>
 int quantize_blocks(const char* what, const void* x, int64_t x_stride, int dtype, int64_t M, int K, uint8_t* out,
@@ -439,8 +480,9 @@ int quantize_blocks(const char* what, const void* x, int64_t x_stride, int dtype
   SB_CHECK_ARG((uintptr_t)x % size == 0 && (uintptr_t)scales % 4 == 0, "%s: x and scales must be aligned to their elements",
                what);
   const int groups = ceil_div(K, kGroup);
-  // Vector accesses need every row (and the gate half) on a boundary of four elements.
-  const bool vec = K % 4 == 0 && x_stride % 4 == 0 && (uintptr_t)x % (4 * size) == 0 && (uintptr_t)out % 4 == 0;
+  // Elements per access: every row (and the gate half) starts on that boundary.
+  auto wide = [&](int n) { return K % n == 0 && fits(n, x, size, x_stride) && fits(n, out, 1); };
+  const int n = wide(4) ? 4 : wide(2) ? 2 : 1;
   cudaStream_t s = (cudaStream_t)stream;
   // Few rows: one group per warp, for the most warps; otherwise four loads in flight per lane.
   const bool four = groups >= 4 && M * groups >= 4096;
@@ -451,8 +493,12 @@ int quantize_blocks(const char* what, const void* x, int64_t x_stride, int dtype
   const dim3 grid((unsigned)((M + rows - 1) / rows), (unsigned)ceil_div(parts, 8));
   auto launch = [&](auto element) {
     using T = decltype(element);
-    auto kernel = four ? (vec ? quantize_blocks_kernel<T, ACT, 4, true> : quantize_blocks_kernel<T, ACT, 4, false>)
-                       : (vec ? quantize_blocks_kernel<T, ACT, 1, true> : quantize_blocks_kernel<T, ACT, 1, false>);
+    auto kernel = four ? (n == 4   ? quantize_blocks_kernel<T, ACT, 4, 4>
+                          : n == 2 ? quantize_blocks_kernel<T, ACT, 4, 2>
+                                   : quantize_blocks_kernel<T, ACT, 4, 1>)
+                       : (n == 4   ? quantize_blocks_kernel<T, ACT, 1, 4>
+                          : n == 2 ? quantize_blocks_kernel<T, ACT, 1, 2>
+                                   : quantize_blocks_kernel<T, ACT, 1, 1>);
     kernel<<<grid, kQuantThreads, 0, s>>>((const T*)x, x_stride, M, groups, K, row_shift, out, scales);
   };
   if (dtype == SB_BF16)
@@ -529,18 +575,21 @@ extern "C" int sb_fp8_add_rms_norm_quantize(const void* x, int64_t x_stride, con
   p.C = C;
   p.groups = ceil_div(C, kGroup);
   p.eps = eps;
-  const uintptr_t row_bytes = 4 * size;
-  p.vec = C % 4 == 0 && x_stride % 4 == 0 && (uintptr_t)x % row_bytes == 0 && (uintptr_t)out % 4 == 0 &&
-          (residual == nullptr || (residual_stride % 4 == 0 && (uintptr_t)residual % row_bytes == 0 &&
-                                   (uintptr_t)summed % row_bytes == 0));
-  p.vec = p.vec && (gate == nullptr || (aligned16(gate) && gate_stride % 4 == 0)) &&
-          (weight == nullptr || (aligned16(weight) && weight_stride % 4 == 0)) &&
-          (shift == nullptr || (aligned16(shift) && shift_stride % 4 == 0));
-  cudaStream_t s = (cudaStream_t)stream;
+  auto wide = [&](int n) {
+    return C % n == 0 && fits(n, x, size, x_stride) && fits(n, residual, size, residual_stride) && fits(n, summed, size) &&
+           fits(n, out, 1) && fits(n, gate, 4, gate_stride) && fits(n, weight, 4, weight_stride) &&
+           fits(n, shift, 4, shift_stride);
+  };
+  const int n = wide(4) ? 4 : wide(2) ? 2 : 1;  // elements per access
+  auto dispatch = [&](auto element) {
+    using T = decltype(element);
+    auto run = n == 4 ? dispatch_norm<T, 4> : n == 2 ? dispatch_norm<T, 2> : dispatch_norm<T, 1>;
+    run(p, blocks != 0, (cudaStream_t)stream);
+  };
   if (dtype == SB_BF16)
-    dispatch_norm<__nv_bfloat16>(p, blocks != 0, s);
+    dispatch(__nv_bfloat16{});
   else
-    dispatch_norm<float>(p, blocks != 0, s);
+    dispatch(float{});
   SB_CHECK_LAUNCH("sb_fp8_add_rms_norm_quantize launch");
   return SB_OK;
 }

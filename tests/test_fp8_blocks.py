@@ -174,7 +174,7 @@ def check_quantised(codes, scale, y, y_error):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("act", ["none", "swiglu", "gelu"])
-@pytest.mark.parametrize("M,K", [(1, 1), (1, 128), (3, 129), (5, 1000), (2, 4104), (517, 136), (1, 14336), (67, 8192)])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 128), (3, 129), (5, 1000), (2, 4104), (517, 136), (1, 14336), (67, 8192), (40, 130), (33, 2490)])
 def test_quantisers_match_their_definition(cuda_device, dtype, act, M, K):
     g = torch.Generator(device=cuda_device).manual_seed(M * 10007 + K)
     call, formula = ACTIVATIONS[act]
@@ -198,7 +198,7 @@ def test_quantisers_read_strided_and_misaligned_rows(cuda_device, act):
     call, _ = ACTIVATIONS[act]
     halves = 2 if act == "swiglu" else 1
     base = torch.randn(40, 2100, device=cuda_device, dtype=torch.bfloat16)
-    for view in (base[:, 8:8 + 256 * halves], base[:, 3:3 + 200 * halves], base[::3, :128 * halves],
+    for view in (base[:, 8:8 + 256 * halves], base[:, 3:3 + 200 * halves], base[:, 2:2 + 256 * halves], base[::3, :128 * halves],
                  base.t()[:130, :40 // halves * halves], base[:1].expand(6, 2100), base.view(-1)[5:5 + 32 * 512].view(32, 512)):
         want = call(view.clone(memory_format=torch.contiguous_format))
         got = call(view)
@@ -256,7 +256,8 @@ def norm_reference(x, weight, residual, gate, shift, eps):
     (1, 4096, True, False, False, 1), (1, 1, False, False, False, 1), (6, 128, True, True, True, 3),
     (259, 5376, True, False, True, 1), (4, 257, True, True, True, 2), (33, 1000, False, False, True, 1),
     (2, 16384, True, True, True, 2), (3, 9911, True, True, False, 1), (700, 1024, True, False, False, 1),
-    (9, 2048, False, False, False, 1), (1200, 4096, True, True, True, 2), (5, 8192, True, True, True, 5)])
+    (9, 2048, False, False, False, 1), (1200, 4096, True, True, True, 2),
+    (6, 130, True, True, True, 3), (40, 2490, True, True, True, 2), (3, 12942, True, False, True, 1), (5, 8192, True, True, True, 5)])
 def test_add_rms_norm_quantize(cuda_device, dtype, blocks, M, C, residual, gate, shift, samples):
     g = torch.Generator(device=cuda_device).manual_seed(M * 31 + C)
 
