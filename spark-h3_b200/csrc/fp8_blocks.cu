@@ -260,8 +260,8 @@ constexpr int norm_ctas(int W, int V) { return (V == 4 ? 512 : 768) / norm_threa
 // stay and walk the rows, R at a time: a row's work is a chain (sum over the CTA, then scale, then
 // codes) of about 2000 cycles, so R rows go through it together, the next R rows in flight
 // (unconverted) meanwhile.  The sum is rounded once, where it is stored; the norm works on the
-// unrounded fp32 sum.  Measured at 124992 x 4096 bf16 with residual, gate and shift (3.6 GB): 583 us,
-// 6.2 TB/s; 64-bit row arithmetic 615, one row at a time 659, one row per CTA without rows in flight
+// unrounded fp32 sum.  Measured at 124992 x 4096 bf16 with residual, gate and shift (3.6 GB): 600 us,
+// 6.0 TB/s; 64-bit row arithmetic 615, one row at a time 659, one row per CTA without rows in flight
 // 832, access-by-access alignment checks instead of the template's 746.
 template <typename T, int W, int V, int R, bool BLOCKS, int N>
 __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm_quantize_kernel(NormParams p) {
@@ -288,12 +288,9 @@ __global__ void __launch_bounds__(norm_threads(W), norm_ctas(W, V)) add_rms_norm
     }
   };
   auto params = [&](const float* base, int64_t at, int j, float fill, float* v) {
-    if (base != nullptr) {
-      load_cols<N>(base + at, c0 + j * W * kGroup, p.C, v);
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fill;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = fill;
+    if (base != nullptr) load_cols<N>(base + at, c0 + j * W * kGroup, p.C, v);
   };
   // The rows only go forward, so a sample is looked up (a division) only past the last one's end.
   const uint32_t per_sample = (uint32_t)p.rows_per_sample;
