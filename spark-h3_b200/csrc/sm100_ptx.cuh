@@ -62,35 +62,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return mbar_wait_limit(bar, parity, abort_flag, status, site, kWaitLimit);
 }
 
-__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// mbar_wait that polls without suspending the thread, for a wait on a short critical path.
-__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                          int site) {
-  if (mbar_test_wait(bar, parity)) return true;
-  const long long start = clock64();
-  for (int n = 1;; ++n) {
-    if (mbar_test_wait(bar, parity)) return true;
-    if ((n & 63) == 0) {
-      if (*abort_flag) return false;
-      if (clock64() - start > kWaitLimit) {
-        *abort_flag = 1;
-        if (status) atomicExch(status, site);
-        return false;
-      }
-    }
-  }
-}
-
 // Bounded wait that ignores the abort flag: used to drain in-flight copies and MMAs
 // before a CTA exits, so nothing lands in shared or tensor memory after it is gone.
 __device__ __forceinline__ bool mbar_drain(uint32_t bar, uint32_t parity) {
