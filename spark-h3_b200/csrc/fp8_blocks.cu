@@ -6,7 +6,7 @@
 // one warp-wide reduction instruction.  What bounds these kernels is HBM once the instructions per
 // value are few: at 6.5 TB/s an SM issues about 17 per bf16 value in the time that its three bytes
 // take.  124992 x 4096 bf16: 232 us, 6.6 TB/s (half a warp per group with shuffles, 64-bit index
-// divisions and exact divisions: 341); SwiGLU of 124992 x 2 x 2048: 222 us, 5.8 TB/s; GELU: 444 us,
+// divisions and exact divisions: 341); SwiGLU of 124992 x 2 x 2048: 226 us, 5.7 TB/s; GELU: 444 us,
 // bound by its instructions.
 //
 // Scales and special values follow torch's spelling of the same arithmetic: scale =
@@ -139,9 +139,12 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int c, int cols, const
 
 enum Activation { kNone = 0, kSwiglu = 1, kGelu = 2 };
 
-// a * g * sigmoid(g).  1 + 2^(-g log2 e) may be infinite: its reciprocal is then 0, as in the limit.
+// a * sigmoid(g) * g, in this order: a * g alone may overflow where the value does not, and what
+// underflows in a * sigmoid(g) stays far below the smallest scale.  1 + 2^(-g log2 e) may be infinite:
+// its reciprocal is then 0, as in the limit.  (124992 x 2 x 2048 in 226 us; g * sigmoid(g) first takes two
+// registers more, 34, so that six CTAs share an SM instead of eight: 263.)
 __device__ __forceinline__ float swiglu(float a, float g) {
-  return a * g * reciprocal(1.f + sm100::ex2_approx(g * -kLog2e));
+  return a * reciprocal(1.f + sm100::ex2_approx(g * -kLog2e)) * g;
 }
 
 // x * Phi(x), with Phi(-|x|) from Abramowitz and Stegun 26.2.17 (error below 7.5e-8, as that of
