@@ -137,17 +137,20 @@ def _same_device(index: int, *tensors) -> None:
             raise RuntimeError(f"all tensors must be on the same CUDA device: one is on {t.device}, not cuda:{index}")
 
 
-def _refuse_overlap(out: torch.Tensor, **inputs) -> None:
-    """An output may be an input itself, laid out alike, but not overlap one in any other way: the
-    kernels read some rows after they have written others."""
+def _refuse_overlap(out: torch.Tensor, in_place: dict, **inputs) -> None:
+    """An output may be one of `in_place` itself, laid out alike: each thread reads those at the
+    places that it writes, before it writes them.  Beyond that it overlaps no input, since other
+    threads still read it after the first have written."""
     first, last = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
-    for name, t in inputs.items():
+    for name, t in {**in_place, **inputs}.items():
         if t is None or t.numel() == 0 or out.numel() == 0:
             continue
-        same = t.data_ptr() == first and t.dtype == out.dtype and t.shape == out.shape and t.is_contiguous()
+        if name in in_place and (t.data_ptr() == first and t.dtype == out.dtype and t.shape == out.shape
+                                 and t.is_contiguous()):
+            continue
         span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
-        if not same and t.data_ptr() < last and first < t.data_ptr() + span * t.element_size():
-            raise ValueError(f"out overlaps {name} without being it")
+        if t.data_ptr() < last and first < t.data_ptr() + span * t.element_size():
+            raise ValueError(f"out overlaps {name}" + (" without being it" if name in in_place else ""))
 
 
 def _call_on(index: int, name: str, *args) -> None:
@@ -229,8 +232,8 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
     or [S, C] with one row per sample (S divides M; row m belongs to sample m // (M / S)).
     Returns (codes [M, C], scales, s): scales [M, ceil(C / 128)] (`blocks`, for fp8_gemm_blocks)
     or [M, 1] (for fp8_gemm); s in x's dtype, written to `out` when given (which may be the
-    residual itself: the residual stream updated in place), or None without a residual.  The
-    norm works on the unrounded fp32 sum.  Outputs carry no gradient."""
+    residual itself, the residual stream updated in place, or x, and overlaps no other input), or
+    None without a residual.  The norm works on the unrounded fp32 sum.  Outputs carry no gradient."""
     x, M, C, x_stride = _strided_rows(x, "x")
     device, dtype = x.device, _dtype_code(x)
     r_stride, residual_ptr, out_ptr = 0, None, None
@@ -247,7 +250,7 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, r
         elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {tuple(x.shape)} {x.dtype}")
         else:
-            _refuse_overlap(out, x=x, residual=residual, weight=weight, gate=gate, shift=shift)
+            _refuse_overlap(out, dict(x=x, residual=residual), weight=weight, gate=gate, shift=shift)
         residual_ptr, out_ptr = residual.data_ptr(), out.data_ptr()
     _same_device(device.index, residual, weight, gate, shift, out)
     samples, gate_ptr, g_stride, weight_ptr, w_stride, shift_ptr, s_stride = 1, None, 0, None, 0, None, 0
@@ -276,8 +279,9 @@ def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Ten
     """[M, N] = a_fp8 [M, K] . b_fp8 [N, K]^T with a_scale [M, ceil(K / 128)] (any strides) applied
     per row and 128 columns and b_scale [ceil(N / 128), ceil(K / 128)] per 128 x 128 block
     (+ bias [N]); residual + gate * (that) with a residual [M, N] of the output's dtype (gate [N],
-    1 when None).  out_dtype bf16 (the default) or fp32; `out` may be the residual itself.  K must
-    be a multiple of 16.  The output carries no gradient."""
+    1 when None).  out_dtype bf16 (the default) or fp32; `out` may be the residual itself and overlaps
+    no other input.  K must be a multiple of 16; the operands, the residual and `out` start on 16
+    bytes.  The output carries no gradient."""
     if a_fp8.dtype != FP8_DTYPE or b_fp8.dtype != FP8_DTYPE:
         raise TypeError("fp8_gemm_blocks takes float8_e4m3fn operands")
     if a_fp8.dim() != 2 or b_fp8.dim() != 2 or a_fp8.shape[1] != b_fp8.shape[1]:
@@ -303,8 +307,8 @@ def fp8_gemm_blocks(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Ten
         if out.shape != (M, N) or out.dtype != out_dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous [{M}, {N}] {out_dtype}")
         _same_device(index, out)
-        _refuse_overlap(out, a_fp8=a_fp8, a_scale=a_scale, b_fp8=b_fp8, b_scale=b_scale, bias=bias, gate=gate,
-                        residual=residual)
+        _refuse_overlap(out, dict(residual=residual), a_fp8=a_fp8, a_scale=a_scale, b_fp8=b_fp8, b_scale=b_scale,
+                        bias=bias, gate=gate)
     code = _dtype_code(out)
     bias_ptr = residual_ptr = gate_ptr = None
     if bias is not None:

@@ -1,5 +1,5 @@
 """Block-scaled e4m3 operators where they meet the edges of their arithmetic and of their arguments:
-SwiGLU of values whose product overflows."""
+SwiGLU of values whose product overflows, outputs that are inputs."""
 from __future__ import annotations
 
 import pytest
@@ -27,3 +27,40 @@ def test_swiglu_of_values_whose_product_overflows(cuda_device, dtype, K):
     y = a * (g * torch.sigmoid(g))
     # exp's argument is off by |g| 2^-23, its value by 2^-22, four more operations by 2^-23 each
     check_quantised(*fl.swiglu_quantize_blocks(h), y, y.abs() * (g.abs() * 2.0 ** -23 + 2.0 ** -20))
+
+
+# ------------------------------------------------------------------------------ outputs that are inputs
+
+@pytest.mark.gpu
+def test_out_is_no_operand_that_others_still_read(cuda_device):
+    x = torch.randn(4, 256, device=cuda_device)
+    for name in ("weight", "shift", "gate"):
+        vec = torch.randn(4, 256, device=cuda_device)  # one sample per row: out's shape and type
+        kept = vec.clone()
+        with pytest.raises(ValueError, match=f"overlaps {name}"):
+            fl.add_rms_norm_quantize(x, residual=x, out=vec, **{name: vec})
+        assert torch.equal(vec, kept)
+    a = torch.ones(4, 512, device=cuda_device).to(fl.FP8_DTYPE)
+    b = torch.ones(4, 512, device=cuda_device).to(fl.FP8_DTYPE)
+    a_scale, b_scale = torch.rand(4, 4, device=cuda_device), torch.rand(1, 4, device=cuda_device)
+    with pytest.raises(ValueError, match="overlaps a_scale"):
+        fl.fp8_gemm_blocks(a, a_scale, b, b_scale, out=a_scale)
+    with pytest.raises(ValueError, match="overlaps b_scale"):
+        fl.fp8_gemm_blocks(a[:1], a_scale[:1], b, b_scale, out=b_scale)
+    row = torch.rand(1, 4, device=cuda_device)
+    with pytest.raises(ValueError, match="overlaps bias"):
+        fl.fp8_gemm_blocks(a[:1], a_scale[:1], b, b_scale, row, out=row)
+    with pytest.raises(ValueError, match="overlaps gate"):
+        fl.fp8_gemm_blocks(a[:1], a_scale[:1], b, b_scale, residual=torch.rand(1, 4, device=cuda_device), gate=row, out=row)
+
+
+def test_only_inputs_read_in_place_may_be_the_output():
+    out = torch.zeros(4, 8)
+    fl._refuse_overlap(out, dict(x=out, residual=None), weight=torch.zeros(8))
+    fl._refuse_overlap(out, dict(x=torch.zeros(4, 8)))
+    with pytest.raises(ValueError, match="overlaps weight$"):
+        fl._refuse_overlap(out, dict(x=out), weight=out)
+    with pytest.raises(ValueError, match="overlaps shift$"):
+        fl._refuse_overlap(out, dict(x=out), shift=out[3])
+    with pytest.raises(ValueError, match="overlaps x without being it"):
+        fl._refuse_overlap(out, dict(x=out.as_strided((4, 8), (1, 4))))
