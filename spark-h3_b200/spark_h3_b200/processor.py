@@ -175,13 +175,15 @@ class _H3SparseProcessor:
     @staticmethod
     def _project(attn, hidden_states, rotary_emb):
         """Q/K/V projections, per-head norms and rotary embedding (processor.py:896-933)."""
+        projected = None
         if getattr(attn, "fused_projections", False):
-            query, key, value = attn.to_qkv(hidden_states).chunk(3, dim=-1)
+            projected = attn.to_qkv(hidden_states).chunk(3, dim=-1)
         elif hasattr(attn.to_q, "forward_quantized"):
             from .fp8_linear import forward_qkv_shared
-            query, key, value = forward_qkv_shared(attn, hidden_states)
-        else:
-            query, key, value = attn.to_q(hidden_states), attn.to_k(hidden_states), attn.to_v(hidden_states)
+            projected = forward_qkv_shared(attn, hidden_states)
+        if projected is None:  # bf16 linears, or fp8 beside other ones
+            projected = attn.to_q(hidden_states), attn.to_k(hidden_states), attn.to_v(hidden_states)
+        query, key, value = projected
         query = attn.norm_q(query.unflatten(-1, (attn.heads, -1)))
         key = attn.norm_k(key.unflatten(-1, (attn.heads, -1)))
         value = value.unflatten(-1, (attn.heads, -1))

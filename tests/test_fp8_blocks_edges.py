@@ -1,11 +1,14 @@
 """Block-scaled e4m3 operators where they meet the edges of their arithmetic and of their arguments:
-SwiGLU of values whose product overflows, outputs that are inputs."""
+SwiGLU of values whose product overflows, outputs that are inputs,
+linears of different kinds side by side."""
 from __future__ import annotations
 
 import pytest
 import torch
+import torch.nn as nn
 
 from spark_h3_b200 import fp8_linear as fl
+from spark_h3_b200.processor import _H3SparseProcessor
 from test_fp8_blocks import check_quantised
 
 
@@ -64,3 +67,51 @@ def test_only_inputs_read_in_place_may_be_the_output():
         fl._refuse_overlap(out, dict(x=out), shift=out[3])
     with pytest.raises(ValueError, match="overlaps x without being it"):
         fl._refuse_overlap(out, dict(x=out.as_strided((4, 8), (1, 4))))
+
+
+# ------------------------------------------------------------------------------ mixed projections
+
+class Attention(nn.Module):
+    """What the sparse processor's projections read of an attention module."""
+
+    def __init__(self, hidden, heads):
+        super().__init__()
+        self.heads, self.fused_projections = heads, False
+        self.to_q, self.to_k, self.to_v = (nn.Linear(hidden, hidden, bias=False) for _ in range(3))
+        self.norm_q = self.norm_k = nn.Identity()
+
+
+class HostFp8Linear(fl.Fp8Linear):
+    """An Fp8Linear whose product is taken on the CPU from its codes and scales."""
+
+    def forward(self, x):
+        return x @ (self.weight_fp8.float() * self.weight_scale.reshape(-1, 1)).T
+
+
+@pytest.mark.parametrize("which", [("to_q",), ("to_q", "to_v"), ("to_k",), ()])
+def test_sparse_processor_projects_fp8_beside_plain_linears(which):
+    torch.manual_seed(6)
+    attn = Attention(32, 2)
+    for name in which:
+        setattr(attn, name, HostFp8Linear(getattr(attn, name)))
+    x = torch.randn(1, 7, 32)
+    with torch.no_grad():
+        got = _H3SparseProcessor._project(attn, x, None)
+        for t, linear in zip(got, (attn.to_q, attn.to_k, attn.to_v)):
+            assert torch.equal(t, linear(x).unflatten(-1, (2, 16)))
+
+
+@pytest.mark.gpu
+def test_sparse_processor_projects_mixed_granularities(cuda_device):
+    torch.manual_seed(7)
+    attn = Attention(256, 2).to(cuda_device, torch.bfloat16)
+    plain = [m for m in (attn.to_q, attn.to_k, attn.to_v)]
+    attn.to_q, attn.to_k = fl.Fp8Linear(attn.to_q), fl.Fp8BlockLinear(attn.to_k)
+    x = torch.randn(1, 70, 256, device=cuda_device, dtype=torch.bfloat16)
+    with torch.no_grad():
+        got = _H3SparseProcessor._project(attn, x, None)
+        for t, linear, before in zip(got, (attn.to_q, attn.to_k, attn.to_v), plain):
+            assert torch.equal(t, linear(x).unflatten(-1, (2, 128)))
+            # two roundings to e4m3 (2^-4 of a value at most): root mean square below 2^-4 together
+            want = before(x).float().flatten()
+            assert float((t.float().flatten() - want).norm() / want.norm()) <= 2.0 ** -4
