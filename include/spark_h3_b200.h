@@ -389,10 +389,11 @@ int sb_fp8_quantize_segments(const void* x, int64_t M, int K, int seg, int64_t s
  * scales are per token or per tensor): for columns [128 b, 128 b + 128) of row m (the last block
  * may be short), scales[m, b] = max(absmax * fp32(1/448), 1e-12) and out = e4m3(y / scale),
  * y being x, a * sigmoid(g) * g of a [M, 2K] projection output (value half first; it overflows only
- * where its value does), or GELU(x) (erf form), evaluated in fp32.  The quotient is formed with a
- * reciprocal and is off by less than 2^-22 of itself: a code can be the neighbour of the nearest
- * one where the quotient lies that close to the middle of the two.  A NaN makes its whole block
- * NaN; an infinity makes its block's finite values 0.
+ * where its value does), or GELU(x) = x * Phi(x), evaluated in fp32: SwiGLU to (|g| 2^-23 + 2^-20)
+ * of its value (a sigmoid below 2^-126 counts as 0), GELU to (1.25 x^2 2^-24 + 2^-18) of its value.
+ * The quotient is formed with a reciprocal and is off by less than 2^-22 of itself: a code can be
+ * the neighbour of the nearest one where the quotient lies that close to the middle of the two.
+ * A NaN makes its whole block NaN; an infinity makes its block's finite values 0.
  * x: rows of K (swiglu: 2K) columns, x_stride elements apart (dtype), aligned to its elements;
  * vector loads where K, the stride and the pointers are multiples of four elements.  K <= 2^24.
  * out: [M, K] bytes; scales: [M, ceil(K / 128)] fp32.

@@ -1,5 +1,5 @@
 """Block-scaled e4m3 operators where they meet the edges of their arithmetic and of their arguments:
-SwiGLU of values whose product overflows, outputs that are inputs,
+SwiGLU of values whose product overflows, GELU's negative tail, outputs that are inputs,
 linears of different kinds side by side."""
 from __future__ import annotations
 
@@ -30,6 +30,25 @@ def test_swiglu_of_values_whose_product_overflows(cuda_device, dtype, K):
     y = a * (g * torch.sigmoid(g))
     # exp's argument is off by |g| 2^-23, its value by 2^-22, four more operations by 2^-23 each
     check_quantised(*fl.swiglu_quantize_blocks(h), y, y.abs() * (g.abs() * 2.0 ** -23 + 2.0 ** -20))
+
+
+# ------------------------------------------------------------------------------ GELU
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,K", [(64, 129), (33, 131), (40, 258), (9, 4096)])
+@pytest.mark.parametrize("low,high", [(-6.0, -1.0), (-4.0, -3.0), (-9.0, 9.0)])
+def test_gelu_is_exact_relative_to_its_value(cuda_device, dtype, M, K, low, high):
+    """A group may hold nothing but GELU's negative tail (a short last group often does): its scale
+    and codes need the tail's relative accuracy."""
+    g = torch.Generator(device=cuda_device).manual_seed(K)
+    x = (torch.rand(M, K, device=cuda_device, generator=g) * (high - low) + low).to(dtype)
+    y = x.double() * torch.special.ndtr(x.double())
+    # Phi(-|x|) e^(x^2 / 2) as a polynomial in t: its fit 3e-7, t (off by 2^-24 + 2^-23) three times
+    # that, seven steps of Horner's rule 1.5e-6, two products and ex2 (2^-22): 2.8e-6 < 2^-18.  The
+    # exponent x^2 / 2 is off by two roundings and its constant's, 2.5 x 2^-24 of itself.
+    error = y.abs() * (2.0 ** -18 + x.double().square() * 1.25 * 2.0 ** -24)
+    check_quantised(*fl.gelu_quantize_blocks(x), y, error)
 
 
 # ------------------------------------------------------------------------------ outputs that are inputs
