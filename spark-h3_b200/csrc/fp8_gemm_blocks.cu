@@ -538,7 +538,7 @@ fp8_gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
 // bytes of a weight row with its 16 columns of the M rows, which it keeps as fp32, so weights go
 // from global memory to registers with no staging, and no TMEM, barrier or tensor map has to be
 // set up.  A CTA of 8 warps takes kRows weight rows per row group; `k_warps` warps split K (512
-// columns each at a time) and the sums meet in shared memory.  1 x 4096 x 4096: 5.9 us (swap 7.3).
+// columns each at a time) and the sums meet in shared memory.  1 x 4096 x 4096: 6.7 us (swap 8.5).
 constexpr int kStreamThreads = 256;
 constexpr int kRows = 8;
 
@@ -641,20 +641,28 @@ int sm_count() {
   return sms;
 }
 
-template <typename T>
-int launch_stream(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, cudaStream_t s) {
-  // Warps along K: the fewest passes over K times waves of CTAs (about four CTAs per SM).
-  int k_warps = 1;
+// The split of the stream kernel's warps along K with the fewest passes over K times waves of CTAs, and its
+// time in us, launch included: a fit of the times below, 0 where one pass of one wave does it all.  An
+// SM holds four CTAs for one row (62 registers a thread), two for two (99).
+double stream_shape(int64_t M, int N, int K, int sms, int* k_warps) {
+  const int64_t resident = (int64_t)sms * (M == 1 ? 4 : 2);
   int64_t best = 0;
+  double estimate = 0;
   for (int w = 1; w <= 8; w *= 2) {
-    const int64_t passes = (p.K + 512 * w - 1) / (512 * w);
-    const int64_t ctas = (p.N + kRows * (8 / w) - 1) / (kRows * (8 / w));
-    const int64_t cost = passes * ((ctas + 4 * sm_count() - 1) / (4 * sm_count()));
-    if (w == 1 || cost < best) {
-      best = cost;
-      k_warps = w;
+    const int64_t passes = ((int64_t)K + 512 * w - 1) / (512 * w);
+    const int64_t ctas = ((int64_t)N + kRows * (8 / w) - 1) / (kRows * (8 / w));
+    const int64_t waves = (ctas + resident - 1) / resident;
+    if (w == 1 || passes * waves < best) {
+      best = passes * waves;
+      estimate = best == 1 ? 0 : 2.5 + (waves == 1 ? 3.2 : 4.0) * (double)best;
+      *k_warps = w;
     }
   }
+  return estimate;
+}
+
+template <typename T>
+int launch_stream(const uint8_t* a, const uint8_t* b, int k_warps, const BlockGemmParams& p, cudaStream_t s) {
   const int rows = kRows * (kStreamThreads / 32 / k_warps);
   const unsigned grid = (unsigned)((p.N + rows - 1) / rows);
   if (p.M == 1)
@@ -1114,14 +1122,19 @@ double swap_shape(int64_t M, int N, int k_blocks, int sms, SwapShape* shape) {
 
 template <typename T>
 int dispatch(const uint8_t* a, const uint8_t* b, const BlockGemmParams& p, cudaStream_t s) {
-  // One or two rows: streaming starts sooner, swap reads faster (256-byte bursts by TMA).  Measured
-  // at one row (stream, swap): 1024 x 1024 3.3, 5.8; 4096 x 4096 5.9, 7.3; 4096 x 16384 18.3, 16.6;
-  // 14336 x 5376 24.5, 16.9; 28672 x 5376 42.4, 28.5.
-  if (p.M <= 2 && (int64_t)p.N * p.K <= (24 << 20)) return launch_stream<T>(a, b, p, s);
   const int sms = sm_count();
   SwapShape q{};
-  const double pair = pair_estimate(p.M, p.N, p.k_blocks, sms);
-  if (swap_shape(p.M, p.N, p.k_blocks, sms, &q) < pair) {
+  const double pair = pair_estimate(p.M, p.N, p.k_blocks, sms), swap = swap_shape(p.M, p.N, p.k_blocks, sms, &q);
+  // One or two rows: streaming starts sooner, swap reads faster (256-byte bursts by TMA).  Measured (stream,
+  // swap; us, in a graph, weights from HBM): one row in one pass 4096 x 1024 5.6, 6.0; 4096 x 4096 6.7, 8.5;
+  // in more 5376 x 4096 9.9, 10.5; 512 x 16384 14.9, 8.7; two rows in one pass 2048 x 4096 6.1, 11.9; in
+  // more 2000 x 8192 9.7, 14.0; 8192 x 2048 10.3, 8.4; 4096 x 5376 17.2, 9.7.  Larger weights, one row:
+  // 4096 x 16384 18.3, 16.6; 28672 x 5376 42.4, 28.5.
+  int k_warps = 1;
+  if (p.M <= 2 && (int64_t)p.N * p.K <= (24 << 20) &&
+      stream_shape(p.M, p.N, p.K, sms, &k_warps) < std::min(swap, pair))
+    return launch_stream<T>(a, b, k_warps, p, s);
+  if (swap < pair) {
     if (q.tokens <= 16) return launch_swap<T, 16>(a, b, p, q, s);
     if (q.tokens <= 32) return launch_swap<T, 32>(a, b, p, q, s);
     return launch_swap<T, 64>(a, b, p, q, s);

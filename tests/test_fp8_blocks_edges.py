@@ -1,15 +1,15 @@
 """Block-scaled e4m3 operators where they meet the edges of their arithmetic and of their arguments:
 SwiGLU of values whose product overflows, GELU's negative tail, outputs that are inputs,
-linears of different kinds side by side."""
+linears of different kinds side by side, one and two rows of A on both sides of their kernels' border."""
 from __future__ import annotations
 
 import pytest
 import torch
 import torch.nn as nn
 
-from spark_h3_b200 import fp8_linear as fl
+from spark_h3_b200 import fp8_linear as fl, ops
 from spark_h3_b200.processor import _H3SparseProcessor
-from test_fp8_blocks import check_quantised
+from test_fp8_blocks import assert_gemm, check_quantised, gemm_inputs, gemm_reference
 
 
 # ------------------------------------------------------------------------------ SwiGLU
@@ -134,3 +134,20 @@ def test_sparse_processor_projects_mixed_granularities(cuda_device):
             # two roundings to e4m3 (2^-4 of a value at most): root mean square below 2^-4 together
             want = before(x).float().flatten()
             assert float((t.float().flatten() - want).norm() / want.norm()) <= 2.0 ** -4
+
+
+# ------------------------------------------------------------------------------ one and two rows
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (1, 5376, 4096), (1, 4096, 4112), (1, 23000, 1024), (1, 512, 16384),
+                                   (2, 2048, 4096), (2, 2368, 4096), (2, 2369, 4096), (2, 4096, 4096), (2, 8192, 2048),
+                                   (2, 1536, 16384), (2, 7, 4112), (1, 1, 8208), (2, 40000, 16), (1, 40000, 16)])
+def test_one_and_two_rows_at_the_border_of_their_kernels(cuda_device, M, N, K):
+    a, a_scale, b, b_scale, g = gemm_inputs(M, N, K, cuda_device, N + K)
+    want, error = gemm_reference(a, a_scale, b, b_scale)
+    assert_gemm(fl.fp8_gemm_blocks(a, a_scale, b, b_scale, out_dtype=torch.float32), want, error)
+    residual = torch.randn(M, N, device=cuda_device, generator=g).to(torch.bfloat16)
+    full = residual.double() + want
+    out = fl.fp8_gemm_blocks(a, a_scale, b, b_scale, residual=residual, out=residual)
+    assert_gemm(out, full, error + full.abs() * 2.0 ** -23)
+    assert ops.read_device_status(cuda_device) == 0
