@@ -51,6 +51,24 @@ def test_gelu_is_exact_relative_to_its_value(cuda_device, dtype, M, K, low, high
     check_quantised(*fl.gelu_quantize_blocks(x), y, error)
 
 
+# ------------------------------------------------------------------------------ the same call again
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [fl.quantize_blocks, fl.swiglu_quantize_blocks, fl.gelu_quantize_blocks])
+def test_quantisers_give_the_same_bits_again(cuda_device, act):
+    """Whichever stream, address and number of rows beside them: a row's codes and scales are its own."""
+    x = torch.randn(259, 2 * 1432, device=cuda_device).to(torch.bfloat16)
+    codes, scale = act(x)
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream(cuda_device))
+    with torch.cuda.stream(side):
+        others = [act(x), act(x.clone()), act(x[:3]), act(torch.nn.functional.pad(x, (1, 0))[:, 1:])]
+    torch.cuda.current_stream(cuda_device).wait_stream(side)
+    for got in others:
+        rows = got[0].shape[0]
+        assert torch.equal(got[0].view(torch.uint8), codes[:rows].view(torch.uint8)) and torch.equal(got[1], scale[:rows])
+
+
 # ------------------------------------------------------------------------------ outputs that are inputs
 
 @pytest.mark.gpu
