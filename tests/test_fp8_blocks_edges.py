@@ -1,13 +1,17 @@
 """Block-scaled e4m3 operators where they meet the edges of their arithmetic and of their arguments:
 SwiGLU of values whose product overflows, GELU's negative tail, outputs that are inputs,
-linears of different kinds side by side, one and two rows of A on both sides of their kernels' border."""
+linears of different kinds side by side, one and two rows of A on both sides of their kernels' border, and the registers that
+the kernels' launches count on."""
 from __future__ import annotations
+
+import re
+import subprocess
 
 import pytest
 import torch
 import torch.nn as nn
 
-from spark_h3_b200 import fp8_linear as fl, ops
+from spark_h3_b200 import _build, fp8_linear as fl, ops
 from spark_h3_b200.processor import _H3SparseProcessor
 from test_fp8_blocks import assert_gemm, check_quantised, gemm_inputs, gemm_reference
 
@@ -169,3 +173,23 @@ def test_one_and_two_rows_at_the_border_of_their_kernels(cuda_device, M, N, K):
     out = fl.fp8_gemm_blocks(a, a_scale, b, b_scale, residual=residual, out=residual)
     assert_gemm(out, full, error + full.abs() * 2.0 ** -23)
     assert ops.read_device_status(cuda_device) == 0
+
+
+# ------------------------------------------------------------------------------ registers
+
+def test_kernels_have_the_registers_that_their_launches_count_on(tmp_path):
+    """The pair kernel refuses to run with another count than the one its warps redistribute, and the
+    choice of the streaming kernel counts four CTAs per SM for one row, two for two."""
+    source = _build.CSRC_DIR / "fp8_gemm_blocks.cu"
+    log = subprocess.run([_build._nvcc(), *_build.NVCC_FLAGS, "-I", str(_build.INCLUDE_DIR), "-Xptxas", "-v", "-c",
+                          str(source), "-o", str(tmp_path / "out.o")], capture_output=True, text=True, check=True).stderr
+    used = {name: int(count) for name, count in
+            re.findall(r"entry function '([^']+)'.*?Used (\d+) registers", log, flags=re.S)}
+    launch = int(re.search(r"kLaunchRegs = (\d+)", source.read_text()).group(1))
+    pair = [n for name, n in used.items() if "pair_kernel" in name]
+    assert len(pair) == 2 and set(pair) == {launch}
+    for rows, resident in ((1, 4), (2, 2)):
+        stream = [n for name, n in used.items() if "stream_kernel" in name and f"Li{rows}E" in name]
+        assert len(stream) == 2
+        for n in stream:  # registers come in eights per thread, 65,536 to an SM
+            assert 65536 // (-(-n // 8) * 8 * 256) == resident
