@@ -1,6 +1,7 @@
 // e4m3 quantisers with one scale per row and 128 columns, and the fused residual + RMSNorm +
 // quantiser.  Each value is read once and kept in registers between the reduction that fixes
-// its scale and the store of its code.
+// its scale and the store of its code (norm rows of more than 8192 fp32 columns spill up to 280 bytes
+// per thread).
 //
 // A warp holds a group of 128 columns, four consecutive ones per lane, so the group's maximum is
 // one warp-wide reduction instruction.  What bounds these kernels is HBM once the instructions per
