@@ -193,3 +193,33 @@ def test_kernels_have_the_registers_that_their_launches_count_on(tmp_path):
         assert len(stream) == 2
         for n in stream:  # registers come in eights per thread, 65,536 to an SM
             assert 65536 // (-(-n // 8) * 8 * 256) == resident
+
+
+# ------------------------------------------------------------------------------ infinities and NaN
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_activations_of_infinities_and_nan(cuda_device, dtype):
+    """A NaN takes its group of 128, an infinity its group's finite values; the other groups stay."""
+    x = torch.randn(6, 300, device=cuda_device).to(dtype)
+    x[0, 130], x[1, 5], x[2, 299] = float("nan"), float("inf"), float("-inf")
+    x[3, 0], x[4, 0] = 3e38, -3e38
+    codes, scale = fl.gelu_quantize_blocks(x)
+    clean = fl.gelu_quantize_blocks(x.nan_to_num(1.0, 1.0, 1.0))
+    assert bool(codes[0, 128:256].float().isnan().all()) and bool(scale[0, 1].isnan())
+    assert bool(scale[1, 0].isinf()) and bool(codes[1, 5].float().isnan())
+    assert bool((codes[1, :128].float().nan_to_num(0.0) == 0).all())
+    assert bool(codes[2, 256:].float().isnan().all())  # -inf * Phi(-inf) is no number, as in torch
+    assert bool(scale[3, 0] > 6e35) and bool((codes[4, 0].float() == 0))
+    hit = torch.zeros(6, 3, dtype=torch.bool, device=cuda_device)
+    hit[0, 1] = hit[1, 0] = hit[2, 2] = True
+    assert torch.equal(scale[~hit], clean[1][~hit])
+    h = torch.randn(4, 600, device=cuda_device).to(dtype)
+    h[0, 3], h[1, 300 + 140], h[2, 7], h[2, 300 + 7] = float("nan"), float("nan"), float("inf"), 1.0
+    h[3, 9], h[3, 300 + 9] = 1.0, float("inf")
+    codes, scale = fl.swiglu_quantize_blocks(h)
+    assert bool(codes[0, :128].float().isnan().all()) and bool(codes[1, 128:256].float().isnan().all())
+    assert not bool(codes[0, 128:].float().isnan().any()) and not bool(codes[1, :128].float().isnan().any())
+    for row, column in ((2, 7), (3, 9)):
+        assert bool(scale[row, 0].isinf()) and bool(codes[row, column].float().isnan())
+        assert bool((codes[row, :128].float().nan_to_num(0.0) == 0).all()) and bool(scale[row, 1:].isfinite().all())
